@@ -346,6 +346,79 @@ ZMI_API int32_t zmi_moe_router_topk(const void *logits, int32_t logits_dt, int64
                             int32_t T, int32_t E, int32_t topk, int32_t renormalize,
                             int32_t *topk_ids, float *topk_weights);
 
+/* zmi_moe_router_grouped: the same step for models that choose their experts by other scores than a softmax's, with
+ * a bias, or within groups of experts (no counterpart in the reference either).  For every token, with x_e its logits:
+ *   scores:  s_e = softmax(x)_e or sigmoid(x_e)   (a logit of -inf has the score 0 whatever the others are);
+ *   choice:  v_e = s_e + bias[e] (bias null: s_e) -- the bias counts for the choice only, not for the weights;
+ *   groups:  n_group > 1: experts [g E/n_group, (g+1) E/n_group) are group g, its value the largest v of its experts
+ *            (ZMI_GROUP_MAX) or the sum of its two largest (ZMI_GROUP_TOP2_SUM); only the experts of the topk_group
+ *            groups of largest value can be chosen;
+ *   ids:     the topk largest v in descending order, equal values (of experts or groups) in ascending order, NaN
+ *            behind everything else; the order is that of values computed in 64 bits;
+ *   weights: s of the chosen experts in that order, with renormalize != 0 divided by their sum (a zero sum leaves
+ *            zeros), times scale.  A NaN logit makes the weights that it enters NaN.
+ * Without a bias and groups valued by their sum the order is the logits' own, so scores that round to one value are
+ * still told apart.  T == 0 is an empty batch: success.
+ * Limits: E <= 512, E a multiple of n_group, n_group <= 64, topk <= min(64, topk_group * E / n_group);
+ * ZMI_GROUP_TOP2_SUM needs groups of two experts or more. */
+enum zmi_router_scoring { ZMI_SCORE_SOFTMAX = 0, ZMI_SCORE_SIGMOID = 1 };
+enum zmi_router_group_score { ZMI_GROUP_MAX = 0, ZMI_GROUP_TOP2_SUM = 1 };
+typedef struct zmi_moe_router_t {
+  int32_t T, E, topk;
+  const void *logits; int32_t logits_dt;    /* f32, bf16 or f16 [T, ldl], device */
+  int64_t ldl;                              /* row stride in elements, >= E */
+  int32_t scoring;                          /* enum zmi_router_scoring */
+  const float *bias;                        /* [E] f32, device, or null */
+  int32_t n_group, topk_group;              /* 1, 1: no groups */
+  int32_t group_score;                      /* enum zmi_router_group_score */
+  int32_t renormalize;
+  float scale;
+  int32_t *topk_ids;                        /* [T, topk] s32, device */
+  float *topk_weights;                      /* [T, topk] f32, device */
+} zmi_moe_router_t;
+/* n_group = topk_group = 1, scale = 1, f32 logits; everything else zero. */
+ZMI_API void zmi_moe_router_params_init(zmi_moe_router_t *r);
+ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
+
+/* zmi_lora_direct: low-rank adapters of many requests at once beside a shared projection (matmul_direct computes the
+ * projection; the reference has no counterpart).  Adapters live in n_slots slots of up to `rank` rows; row t of the
+ * batch uses slot a = slot_ids[t].  For every slice s of the projection's columns (a fused query / key / value or
+ * gate / up projection has several; slice s covers N[s] columns behind those of the slices before it):
+ *   h[r]      = sum_k x[t][k] * A[a][s * rank + r][k],                            r < ranks[a]
+ *   dst[t][n] = base[t][n] + scales[a] * sum_r h[r] * B_s[a][n][r]
+ * Sums are f32, h keeps at least 16 bits of its values' precision in front of the second product, and dst is rounded
+ * once, to nearest even.  base may be dst itself (same pointer and stride: the rows of dst get their adapters' part
+ * added, rows without an adapter are left as they are), another buffer of dst's type, or null (zero).  A slot id outside
+ * [0, n_slots) means no adapter: dst = base.  ranks (null: `rank` for all) holds the rank of the adapter in each slot,
+ * taken as 0 .. rank; what the slot holds beyond it is not used.  scales null: 1.
+ * x, A, B: one type, bf16 or f16; dst (and base): bf16, f16 or f32.
+ * workspace: device memory of zmi_lora_workspace_size() bytes, 16-byte aligned; null: the calling thread's scratch
+ * arena, which a stream that is being captured into a graph cannot use (failure) -- give a captured call a workspace that
+ * no other graph shares.  T == 0 is an empty batch: success.
+ * Limits: rank <= 256, n_slices <= ZMI_LORA_MAX_SLICES, n_slots <= 65535. */
+#define ZMI_LORA_MAX_SLICES 4
+typedef struct zmi_lora_t {
+  int32_t T, K, rank, n_slices, n_slots;
+  int32_t N[ZMI_LORA_MAX_SLICES];
+  int32_t dt_x, dt_dst;
+  const void *x; int64_t ldx;                       /* [T, ldx] */
+  const int32_t *slot_ids;                          /* [T] */
+  const void *a; int64_t a_ld, a_slot;              /* row (n_slices * rank per slot) and slot stride in elements */
+  const void *b[ZMI_LORA_MAX_SLICES];               /* per slice [n_slots][N[s]][rank] */
+  int64_t b_ld[ZMI_LORA_MAX_SLICES], b_slot[ZMI_LORA_MAX_SLICES];
+  const int32_t *ranks;                             /* [n_slots] or null */
+  const float *scales;                              /* [n_slots] or null */
+  const void *base; int64_t ld_base;
+  void *dst; int64_t ld_dst;
+  void *workspace; uint64_t workspace_bytes;
+} zmi_lora_t;
+/* n_slices = 1, bf16 everywhere; everything else zero. */
+ZMI_API void zmi_lora_params_init(zmi_lora_t *l);
+/* Bytes of workspace a call with these sizes (T, K, rank, n_slices, n_slots, N and the types; pointers are not looked
+ * at) needs; 0 for sizes that zmi_lora_direct refuses, and for calls that need none. */
+ZMI_API uint64_t zmi_lora_workspace_size(const zmi_lora_t *l);
+ZMI_API int32_t zmi_lora_direct(const zmi_lora_t *l);
+
 /* zmi_moe_fused_device: whole MoE block with routing kept on the device.
  * x [T,H] bf16 -> per-token s8 quantization -> expert-sorted scatter ->
  * Op1 (gate|up, s8 blob) -> act(gate)*up -> bf16 -> per-token s8 ->

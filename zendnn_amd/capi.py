@@ -28,7 +28,12 @@ ALGO_ONEDNN_BLOCKED, ALGO_LIBXSMM_BLOCKED = 2, 3
 
 ACT_NONE, ACT_SILU_AND_MUL, ACT_GELU_AND_MUL, ACT_SWIGLU_OAI_MUL = range(4)
 
+# zmi_router_scoring, zmi_router_group_score
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2_SUM = 0, 1
+
 MAX_DIMS = 4
+LORA_MAX_SLICES = 4
 
 
 class QuantT(C.Structure):
@@ -134,6 +139,28 @@ class MoeDeviceT(C.Structure):
                 ("out", C.c_void_p), ("ldo", C.c_int32)]
 
 
+class MoeRouterT(C.Structure):
+    _fields_ = [("T", C.c_int32), ("E", C.c_int32), ("topk", C.c_int32),
+                ("logits", C.c_void_p), ("logits_dt", C.c_int32), ("ldl", C.c_int64),
+                ("scoring", C.c_int32), ("bias", C.c_void_p),
+                ("n_group", C.c_int32), ("topk_group", C.c_int32), ("group_score", C.c_int32),
+                ("renormalize", C.c_int32), ("scale", C.c_float),
+                ("topk_ids", C.c_void_p), ("topk_weights", C.c_void_p)]
+
+
+class LoraT(C.Structure):
+    _fields_ = [("T", C.c_int32), ("K", C.c_int32), ("rank", C.c_int32), ("n_slices", C.c_int32),
+                ("n_slots", C.c_int32), ("N", C.c_int32 * LORA_MAX_SLICES),
+                ("dt_x", C.c_int32), ("dt_dst", C.c_int32),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("slot_ids", C.c_void_p),
+                ("a", C.c_void_p), ("a_ld", C.c_int64), ("a_slot", C.c_int64),
+                ("b", C.c_void_p * LORA_MAX_SLICES), ("b_ld", C.c_int64 * LORA_MAX_SLICES),
+                ("b_slot", C.c_int64 * LORA_MAX_SLICES),
+                ("ranks", C.c_void_p), ("scales", C.c_void_p),
+                ("base", C.c_void_p), ("ld_base", C.c_int64), ("dst", C.c_void_p), ("ld_dst", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 # name -> (restype, argtypes); every symbol include/zmi_lowoha.h declares.
 SIGNATURES = {
     "zmi_matmul_params_init": (None, [C.POINTER(MatmulParamsT)]),
@@ -171,6 +198,11 @@ SIGNATURES = {
                                   C.c_void_p, C.c_void_p]),
     "zmi_moe_router_topk": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                         C.c_void_p, C.c_void_p]),
+    "zmi_moe_router_params_init": (None, [C.POINTER(MoeRouterT)]),
+    "zmi_moe_router_grouped": (C.c_int32, [C.POINTER(MoeRouterT)]),
+    "zmi_lora_params_init": (None, [C.POINTER(LoraT)]),
+    "zmi_lora_workspace_size": (C.c_uint64, [C.POINTER(LoraT)]),
+    "zmi_lora_direct": (C.c_int32, [C.POINTER(LoraT)]),
     "zmi_moe_fused_device": (C.c_int32, [C.POINTER(MoeDeviceT)]),
     "zmi_calib_hbm_read": (C.c_int32, [C.POINTER(C.c_void_p), C.c_int32, C.c_uint64, C.c_int32, C.c_int32,
                                        C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_float)]),

@@ -840,6 +840,45 @@ int32_t zmi_moe_router_topk(const void *logits, int32_t logits_dt, int64_t ldl, 
   return ZMI_SUCCESS;
 }
 
+void zmi_moe_router_params_init(zmi_moe_router_t *r) {
+  if (!r) return;
+  std::memset(r, 0, sizeof(*r));
+  r->logits_dt = ZMI_DT_F32;
+  r->n_group = r->topk_group = 1;
+  r->scale = 1.0f;
+}
+
+int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r) {
+  clear_error();
+  if (!r || r->T < 0 || r->E <= 0 || r->topk <= 0 || r->ldl < r->E || r->n_group <= 0) { set_error("moe_router_grouped: bad arguments"); return ZMI_FAILURE; }
+  if (r->E > 512 || r->topk > 64 || r->n_group > 64) { set_error("moe_router_grouped: at most 512 experts, 64 groups and topk <= 64"); return ZMI_UNIMPLEMENTED; }
+  if (r->E % r->n_group) { set_error("moe_router_grouped: the groups must divide the experts"); return ZMI_FAILURE; }
+  const int per = r->E / r->n_group;
+  if (r->topk_group <= 0 || r->topk_group > r->n_group) { set_error("moe_router_grouped: topk_group must be 1 .. n_group"); return ZMI_FAILURE; }
+  if (r->topk > r->topk_group * per) { set_error("moe_router_grouped: topk exceeds the number of experts in topk_group groups"); return ZMI_FAILURE; }
+  if (r->scoring != ZMI_SCORE_SOFTMAX && r->scoring != ZMI_SCORE_SIGMOID) { set_error("moe_router_grouped: scoring must be softmax or sigmoid"); return ZMI_FAILURE; }
+  if (r->group_score != ZMI_GROUP_MAX && r->group_score != ZMI_GROUP_TOP2_SUM) { set_error("moe_router_grouped: unknown group_score"); return ZMI_FAILURE; }
+  if (r->group_score == ZMI_GROUP_TOP2_SUM && r->n_group > 1 && per < 2) { set_error("moe_router_grouped: the sum of a group's two best needs groups of two"); return ZMI_FAILURE; }
+  if (r->logits_dt != ZMI_DT_F32 && r->logits_dt != ZMI_DT_BF16 && r->logits_dt != ZMI_DT_F16) { set_error("moe_router_grouped: logits must be f32, bf16 or f16"); return ZMI_FAILURE; }
+  if (r->T == 0) return ZMI_SUCCESS;
+  if (!r->logits || !r->topk_ids || !r->topk_weights) { set_error("moe_router_grouped: null argument"); return ZMI_FAILURE; }
+  if ((uintptr_t)r->logits % (r->logits_dt == ZMI_DT_F32 ? 4 : 2) || (uintptr_t)r->bias % 4 || (uintptr_t)r->topk_ids % 4 ||
+      (uintptr_t)r->topk_weights % 4) {
+    set_error("moe_router_grouped: an address is not a multiple of its element's size");
+    return ZMI_FAILURE;
+  }
+  note_operand(r->logits); note_operand(r->bias); note_operand(r->topk_ids); note_operand(r->topk_weights);
+  if (!ensure_device()) return ZMI_FAILURE;
+  ZmiRouterGrouped p;
+  p.logits = r->logits; p.ldl = r->ldl; p.bias = r->bias; p.topk_ids = r->topk_ids; p.topk_weights = r->topk_weights;
+  p.logits_dt = r->logits_dt; p.T = r->T; p.E = r->E; p.topk = r->topk; p.n_group = r->n_group; p.topk_group = r->topk_group;
+  p.sigmoid = r->scoring == ZMI_SCORE_SIGMOID; p.top2 = r->group_score == ZMI_GROUP_TOP2_SUM;
+  p.renormalize = r->renormalize != 0; p.scale = r->scale;
+  if (!hip_ok(zmi_launch_moe_router_grouped(p, stream()), "moe router launch")) return ZMI_FAILURE;
+  set_kernel_name("moe_router_grouped");
+  return ZMI_SUCCESS;
+}
+
 int32_t zmi_moe_fused_device(const zmi_moe_device_t *d) {
   clear_error();
   if (!d || !d->x || !d->topk_ids || !d->topk_weights || !d->w13_blob || !d->w2_blob || !d->w13_scale || !d->w2_scale || !d->out) {

@@ -309,6 +309,42 @@ hipError_t zmi_launch_moe_router_topk(const void *logits, int logits_dt, int64_t
 hipError_t zmi_launch_moe_route(const int32_t *topk_ids, int T, int topk, int E, int align, int32_t *counts,
                                 int32_t *offsets, int32_t *slot_of, int32_t *src_of, int n_slots,
                                 int32_t *hist_scratch, hipStream_t stream);
+// k_router_grouped.hip: zmi_moe_router_t with its rules checked
+struct ZmiRouterGrouped {
+  const void *logits;
+  int64_t ldl;
+  const float *bias;          // or null
+  int32_t *topk_ids;
+  float *topk_weights;
+  int32_t logits_dt, T, E, topk, n_group, topk_group;
+  int32_t sigmoid;            // 0: softmax
+  int32_t top2;               // 1: a group's value is the sum of its two best
+  int32_t renormalize;
+  float scale;
+};
+hipError_t zmi_launch_moe_router_grouped(const ZmiRouterGrouped &p, hipStream_t stream);
+
+// k_lora.hip: zmi_lora_t with its rules checked (the operands' meaning is described there)
+struct ZmiLora {
+  const void *x;
+  int64_t ldx;
+  const int32_t *slot_ids;
+  const void *a;
+  int64_t a_ld, a_slot;
+  const void *b[4];
+  int64_t b_ld[4], b_slot[4];
+  const int32_t *ranks;       // or null
+  const float *scales;        // or null
+  const void *base;           // or null; dst: in place
+  int64_t ld_base;
+  void *dst;
+  int64_t ld_dst;
+  float *h;                   // workspace
+  int32_t T, K, rank, n_slices, n_slots, N[4];
+  int32_t dt_x, dt_dst;
+};
+size_t zmi_lora_workspace_bytes(const ZmiLora &p);   // (goes by the sizes and types only)
+hipError_t zmi_launch_lora(const ZmiLora &p, hipStream_t stream, const char **name);
 // A1 is fragment-major over the slot numbering, K_pad = zmi_blob_kpad(H)
 hipError_t zmi_launch_moe_quant_scatter(const void *x, int64_t ldx, int T, int H, int topk,
                                         const int32_t *slot_of, int8_t *A1, float *s1, hipStream_t stream);

@@ -363,6 +363,123 @@ def moe_router_topk(logits, topk, renormalize=False):
     return st, ids, w
 
 
+def _device_rows(name, t, dts, ndim=2):
+    """Data type code of a tensor whose address and strides go to the library: on the GPU, last dimension contiguous."""
+    import torch
+    known = {torch.float32: capi.DT_F32, torch.bfloat16: capi.DT_BF16, torch.float16: capi.DT_F16, torch.int32: DT_S32}
+    dt = known.get(t.dtype)
+    if dt not in dts:
+        raise ValueError(f"{name}: unsupported dtype {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: not on the GPU")
+    if t.dim() != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: {ndim} dimensions with a contiguous last one are required")
+    return dt
+
+
+def _row_stride(t):
+    # (the stride of a dimension of one element is arbitrary in torch: the narrowest valid one then)
+    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+
+
+def prepared_moe_router_grouped(logits, topk, scoring=capi.SCORE_SOFTMAX, bias=None, n_group=1, topk_group=1,
+                                group_score=capi.GROUP_MAX, renormalize=False, scale=1.0):
+    """Flattens the arguments of moe_router_grouped once: returns (call, topk_ids, topk_weights); call() issues the
+    call on the tensors' present contents, writes the two outputs and returns the status.  For serving loops."""
+    import torch
+    dt = _device_rows("logits", logits, (capi.DT_F32, capi.DT_BF16, capi.DT_F16))
+    if bias is not None:
+        _device_rows("bias", bias, (capi.DT_F32,), 1)
+        if bias.device != logits.device or bias.shape[0] != logits.shape[1]:
+            raise ValueError("bias: one value per expert on the logits' device is required")
+    T, E = logits.shape
+    ids = torch.empty(T, max(topk, 0), dtype=torch.int32, device=logits.device)
+    w = torch.empty(T, max(topk, 0), dtype=torch.float32, device=logits.device)
+    r = capi.MoeRouterT()
+    r.T, r.E, r.topk = T, E, topk
+    r.logits, r.logits_dt, r.ldl = logits.data_ptr(), dt, _row_stride(logits)
+    r.scoring, r.bias = scoring, _ptr(bias)
+    r.n_group, r.topk_group, r.group_score = n_group, topk_group, group_score
+    r.renormalize, r.scale = int(bool(renormalize)), scale
+    r.topk_ids, r.topk_weights = ids.data_ptr(), w.data_ptr()
+    fn, ref, keep = capi.load().zmi_moe_router_grouped, C.byref(r), (logits, bias, ids, w)
+    # (the closure holds what the argument block points into)
+    return (lambda _keep=keep: fn(ref)), ids, w
+
+
+def moe_router_grouped(logits, topk, scoring=capi.SCORE_SOFTMAX, bias=None, n_group=1, topk_group=1,
+                       group_score=capi.GROUP_MAX, renormalize=False, scale=1.0):
+    """logits: f32 / bf16 / f16 tensor [T, E] on the GPU, bias: f32 [E] or None -> (status, topk_ids int32 [T, topk],
+    topk_weights f32 [T, topk]); scores, groups and weights as zmi_moe_router_grouped describes them."""
+    call, ids, w = prepared_moe_router_grouped(logits, topk, scoring, bias, n_group, topk_group, group_score, renormalize,
+                                               scale)
+    return call(), ids, w
+
+
+def _lora_args(x, slot_ids, a, b, dst, base, ranks, scales, workspace):
+    half = (capi.DT_BF16, capi.DT_F16)
+    b = list(b) if isinstance(b, (list, tuple)) else [b]
+    if not 1 <= len(b) <= capi.LORA_MAX_SLICES:
+        raise ValueError(f"b: 1 to {capi.LORA_MAX_SLICES} slices")
+    l = capi.LoraT()
+    capi.load().zmi_lora_params_init(C.byref(l))
+    l.dt_x = _device_rows("x", x, half)
+    l.dt_dst = _device_rows("dst", dst, half + (capi.DT_F32,))
+    _device_rows("slot_ids", slot_ids, (DT_S32,), 1)
+    for name, t, nd in [("a", a, 3)] + [("b", t, 3) for t in b]:
+        if _device_rows(name, t, half, nd) != l.dt_x:
+            raise ValueError(f"{name}: the type of x is required")
+    T, K = x.shape
+    S, rank = a.shape[0], b[0].shape[2]
+    if slot_ids.shape[0] != T or a.shape[1] != len(b) * rank or a.shape[2] != K:
+        raise ValueError("slot_ids [T], a [n_slots, n_slices * rank, K] are required")
+    if any(t.shape[0] != S or t.shape[2] != rank for t in b):
+        raise ValueError("b: [n_slots, N, rank] is required")
+    N = [t.shape[1] for t in b]
+    for name, t in (("dst", dst), ("base", base)):
+        if t is not None and (tuple(t.shape) != (T, sum(N)) or _device_rows(name, t, (l.dt_dst,)) != l.dt_dst):
+            raise ValueError(f"{name}: [T, sum of N] of dst's type is required")
+    for name, t, dt in (("ranks", ranks, DT_S32), ("scales", scales, DT_F32)):
+        if t is not None and (_device_rows(name, t, (dt,), 1) != dt or t.shape[0] != S):
+            raise ValueError(f"{name}: [n_slots] is required")
+    for name, t in (("slot_ids", slot_ids), ("a", a), ("dst", dst), ("base", base), ("ranks", ranks), ("scales", scales),
+                    ("workspace", workspace), *(("b", t) for t in b)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: not on the device of x")
+    l.T, l.K, l.rank, l.n_slices, l.n_slots = T, K, rank, len(b), S
+    l.x, l.ldx, l.slot_ids = x.data_ptr(), _row_stride(x), slot_ids.data_ptr()
+    l.a, l.a_ld, l.a_slot = a.data_ptr(), _row_stride(a), a.stride(0) if S > 1 else 0
+    for i, t in enumerate(b):
+        l.N[i], l.b[i], l.b_ld[i], l.b_slot[i] = N[i], t.data_ptr(), _row_stride(t), t.stride(0) if S > 1 else 0
+    l.ranks, l.scales = _ptr(ranks), _ptr(scales)
+    l.dst, l.ld_dst = dst.data_ptr(), _row_stride(dst)
+    if base is not None:
+        l.base, l.ld_base = base.data_ptr(), _row_stride(base)
+    if workspace is not None:
+        l.workspace, l.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return l
+
+
+def lora_workspace_size(x, slot_ids, a, b, dst, base=None, ranks=None, scales=None):
+    """Bytes of workspace that lora_direct with these arguments needs."""
+    return capi.load().zmi_lora_workspace_size(C.byref(_lora_args(x, slot_ids, a, b, dst, base, ranks, scales, None)))
+
+
+def prepared_lora(x, slot_ids, a, b, dst, base=None, ranks=None, scales=None, workspace=None):
+    """Flattens the arguments of lora_direct once and returns call(): the same call on the tensors' present contents,
+    which returns the status.  For serving loops."""
+    l = _lora_args(x, slot_ids, a, b, dst, base, ranks, scales, workspace)
+    fn, ref, keep = capi.load().zmi_lora_direct, C.byref(l), (x, slot_ids, a, b, dst, base, ranks, scales, workspace)
+    return lambda _keep=keep: fn(ref)
+
+
+def lora_direct(x, slot_ids, a, b, dst, base=None, ranks=None, scales=None, workspace=None):
+    """dst[t] = base[t] + scales[s] * (x[t] A[s]^T) B[s]^T with s = slot_ids[t] (dst[t] = base[t] for ids outside the slots).
+    x [T, K], a [n_slots, n_slices * rank, K], b [n_slots, N, rank] or a list of them (the slices of a fused projection),
+    dst [T, sum of N]; base: dst itself (adds in place), another tensor like dst, or None (zero).  Returns the status."""
+    return prepared_lora(x, slot_ids, a, b, dst, base, ranks, scales, workspace)()
+
+
 def moe_fused_device(x, topk_ids, topk_weights, w13_blobs, w2_blobs, w13_scales, w2_scales, I, gated_act, out):
     T, H = x.shape
     E = len(w13_blobs)
