@@ -12,13 +12,14 @@ bool half_type(int32_t dt) { return dt == ZMI_DT_BF16 || dt == ZMI_DT_F16; }
 // The sizes and types alone (what zmi_lora_workspace_size goes by): status, with the error text set when refused.
 int32_t lora_check_sizes(const zmi_lora_t &l) {
   if (l.T < 0 || l.K <= 0 || l.rank <= 0 || l.n_slices <= 0 || l.n_slots <= 0) { set_error("lora: bad sizes"); return ZMI_FAILURE; }
-  if (l.rank > 256 || l.n_slices > ZMI_LORA_MAX_SLICES || l.n_slots > 65535) { set_error("lora: at most rank 256, 4 slices, 65535 slots"); return ZMI_UNIMPLEMENTED; }
+  if (l.rank > 256 || l.n_slices > ZMI_LORA_MAX_SLICES || l.n_slots > ZMI_LORA_MAX_SLOTS) { set_error("lora: at most rank 256, 4 slices, 4096 slots"); return ZMI_UNIMPLEMENTED; }
   int64_t cols = 0;
   for (int s = 0; s < l.n_slices; ++s) {
     if (l.N[s] <= 0) { set_error("lora: bad sizes"); return ZMI_FAILURE; }
     cols += l.N[s];
   }
   if (cols > 0x7fffff00) { set_error("lora: too many columns"); return ZMI_UNIMPLEMENTED; }
+  if (l.T > 1 << 20) { set_error("lora: at most 2^20 rows"); return ZMI_UNIMPLEMENTED; }
   if (!half_type(l.dt_x)) { set_error("lora: dt_x must be bf16 or f16"); return ZMI_UNIMPLEMENTED; }
   if (!half_type(l.dt_dst) && l.dt_dst != ZMI_DT_F32) { set_error("lora: dt_dst must be bf16, f16 or f32"); return ZMI_UNIMPLEMENTED; }
   return ZMI_SUCCESS;
@@ -101,7 +102,7 @@ int32_t zmi_lora_direct(const zmi_lora_t *l) {
       if (!arena().begin(Arena::padded(need))) return ZMI_FAILURE;
       ws = arena().alloc(need);
     }
-    p.h = (float *)ws;
+    p.workspace = ws;
   }
   const char *name = "lora";
   if (!hip_ok(zmi_launch_lora(p, stream(), &name), "lora launch")) return ZMI_FAILURE;

@@ -339,9 +339,20 @@ struct ZmiLora {
   int64_t ld_base;
   void *dst;
   int64_t ld_dst;
-  float *h;                   // workspace
+  void *workspace;            // zmi_lora_workspace_bytes() bytes
   int32_t T, K, rank, n_slices, n_slots, N[4];
   int32_t dt_x, dt_dst;
+};
+#define ZMI_LORA_MAX_SLOTS 4096
+// the parts of the workspace
+struct ZmiLoraPlan {
+  int32_t *header;            // number of tiles
+  int32_t *tiles;             // {slot, first position in `order`, rows, unused} of each
+  int32_t *order;             // [T] rows sorted by slot
+  uint32_t *arrivals;         // a word per tile and group of rank tiles, zeroed by the plan launch
+  void *h;                    // h as MFMA operands
+  float *partial;             // the K slices' sums
+  int32_t n_arrivals;
 };
 size_t zmi_lora_workspace_bytes(const ZmiLora &p);   // (goes by the sizes and types only)
 hipError_t zmi_launch_lora(const ZmiLora &p, hipStream_t stream, const char **name);
