@@ -4,146 +4,303 @@
 //   * group values: the largest v, or the sum of the two largest; the best topk_group groups stay;
 //   * the topk best v among their experts, weights from s.
 //
-// One wavefront per token, 4 tokens per workgroup; lane l holds experts l, l + 64, ... (at most 8).  Two experts of one
-// token can lie nearer to each other than f32 tells apart (256 experts leave gaps of 1e-3 on average, so one token in
-// some thousands has two chosen or bordering values within an f32 ulp), hence scores and values in 64 bits.
+// One wavefront per token, 4 tokens per workgroup; lane l holds experts J l .. J l + J - 1.  A round of the choice is a
+// maximum over the wavefront's keys (DPP, no LDS), a ballot per held expert, and the lowest lane and expert that hold it.
+//
+// Two experts of one token can lie nearer to each other than f32 tells apart (256 experts leave gaps of 1e-3 on average,
+// so one token in some hundreds has two chosen or bordering values within f32's error), and ids have to be those of
+// exact values.  The choice is therefore made on f32 values while every gap that decides it -- between one chosen expert
+// and the next, the last and the best that is left, the last group and the best that is left -- is wider than twice what
+// the f32 values can be off by; a token where one is not is chosen again by the same rounds on 64-bit values.  Without a
+// bias experts are ordered by their logits, exactly, and no score is computed but those of the chosen.
+#include <type_traits>
+
 #include "zmi_device.h"
 #include "zmi_launch.h"
 
 #define RGK_WAVES 4
-#define RGK_PER_LANE 8
 
 namespace {
 
-// double -> unsigned key whose unsigned order is the value order; -0 == +0; NaN lowest
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t rgk_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint64_t rgk_dpp(uint64_t v) {
+  return rgk_dpp<CTRL, ROWS>((uint32_t)v) | (uint64_t)rgk_dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
+}
+
+// maximum over the wavefront (lanes that a step does not reach get 0, the least value)
+__device__ __forceinline__ uint32_t rgk_wave_max(uint32_t v) {
+  v = max(v, rgk_dpp<0x111>(v));        // row_shr 1, 2, 4, 8: lane 15 of each row of 16
+  v = max(v, rgk_dpp<0x112>(v));
+  v = max(v, rgk_dpp<0x114>(v));
+  v = max(v, rgk_dpp<0x118>(v));
+  v = max(v, rgk_dpp<0x142, 0xa>(v));   // row_bcast 15 into rows 1 and 3
+  v = max(v, rgk_dpp<0x143, 0xc>(v));   // row_bcast 31 into rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint64_t rgk_wave_max(uint64_t v) {
+  const uint32_t hi = rgk_wave_max((uint32_t)(v >> 32));
+  return (uint64_t)hi << 32 | rgk_wave_max((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+}
+
+__device__ __forceinline__ double rgk_wave_sum(double v) {
+  auto step = [&](uint64_t u) { v += __longlong_as_double((long long)u); };
+  auto bits = [&] { return (uint64_t)__double_as_longlong(v); };
+  step(rgk_dpp<0x111>(bits()));
+  step(rgk_dpp<0x112>(bits()));
+  step(rgk_dpp<0x114>(bits()));
+  step(rgk_dpp<0x118>(bits()));
+  step(rgk_dpp<0x142, 0xa>(bits()));
+  step(rgk_dpp<0x143, 0xc>(bits()));
+  const uint64_t u = bits();
+  return __longlong_as_double((long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)u, 63) |
+                                          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), 63) << 32));
+}
+
+// value -> unsigned key in the values' order; -0 == +0; NaN 1, below every number (0: nothing)
+__device__ __forceinline__ uint32_t rgk_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return x != x ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
 __device__ __forceinline__ uint64_t rgk_key(double x) {
-  if (x != x) return 0u;
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
-  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+  return x != x ? 1u : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
+__device__ __forceinline__ float rgk_value(uint32_t k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ double rgk_value(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k)); }
 
-// (key, index) of the wavefront's best: largest key, then lowest index; index < 0: nothing to offer
-__device__ __forceinline__ void rgk_best(uint64_t &k, int &i) {
+// One round over the wavefront's J keys a lane: the largest key's first holder (lowest lane, then lowest j) is taken out;
+// returns its expert and, in *best, the key.
+template <int J, class K>
+__device__ __forceinline__ int rgk_take(K (&key)[J], K *best) {
+  K m = key[0];
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) {
-    const uint64_t ok = __shfl_xor((unsigned long long)k, s, 64);
-    const int oi = __shfl_xor(i, s, 64);
-    if (oi >= 0 && (i < 0 || ok > k || (ok == k && oi < i))) { k = ok; i = oi; }
+  for (int j = 1; j < J; ++j) m = max(m, key[j]);
+  const K top = rgk_wave_max(m);
+  uint64_t hit[J], any = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) { hit[j] = __ballot(key[j] == top); any |= hit[j]; }
+  const int lane = __builtin_ctzll(any);
+  uint64_t open = 1ull << lane;
+  int at = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const uint64_t mine = hit[j] & open;
+    if (mine) at = j;
+    open &= ~mine;
+    if ((threadIdx.x % 64) == lane && mine) key[j] = 0;
   }
+  *best = top;
+  return lane * J + at;
 }
 
-__device__ __forceinline__ double rgk_sum(double v) {
+// The two largest of two lanes, from the two largest of each.
+template <int CTRL, class K>
+__device__ __forceinline__ void rgk_pair(K &a, K &b) {
+  const K c = rgk_dpp<CTRL>(a), d = rgk_dpp<CTRL>(b);
+  b = max(min(a, c), max(b, d));
+  a = max(a, c);
+}
+
+// The choice.  key: what experts are ordered by, v: the values that groups are valued by (top2); both of V's type.  V
+// float: false when a gap that decides is not above `gap`.  Lane r gets the r-th expert.
+template <int J, class V, class K>
+__device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J], const V (&v)[J], V gap, void *scratch, int *mine) {
+  const int lane = threadIdx.x % 64, e0 = lane * J, n = p.E - e0, per = p.per;
+  bool sure = true;
+  if (p.topk_group < p.n_group) {
+    K a = 0, b = 0;   // a lane's, then its group's, two largest
+    const bool in_lanes = p.lane_shift >= 0;
+    if (in_lanes) {
+      const int lanes = 1 << p.lane_shift;
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
-  return v;
+      for (int j = 0; j < J; ++j) {
+        const K k = !p.top2 ? key[j] : j < n ? rgk_key(v[j]) : (K)0;
+        b = max(b, min(a, k));
+        a = max(a, k);
+      }
+      // (steps inside rows of 16 lanes: swap neighbours, pairs, mirror halves of eight, mirror the row)
+      if (lanes > 1) rgk_pair<0xb1>(a, b);
+      if (lanes > 2) rgk_pair<0x4e>(a, b);
+      if (lanes > 4) rgk_pair<0x141>(a, b);
+      if (lanes > 8) rgk_pair<0x140>(a, b);
+    } else {
+      K *all = (K *)scratch;
+#pragma unroll
+      for (int j = 0; j < J; ++j) all[e0 + j] = p.top2 ? rgk_key(v[j]) : key[j];
+      // (one wavefront writes and reads its own slice: the order of its LDS instructions is all that is needed)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (lane < p.n_group)
+        for (int i = 0; i < per; ++i) {
+          const K k = all[lane * per + i];
+          b = max(b, min(a, k));
+          a = max(a, k);
+        }
+    }
+    // group g is held by lanes [g << w, (g + 1) << w)
+    const int w = in_lanes ? p.lane_shift : 0, g = lane >> w;
+    K gk = g < p.n_group ? (p.top2 ? rgk_key(rgk_value(a) + rgk_value(b)) : a) : (K)0, last = 0;
+    uint64_t groups = 0;
+    for (int r = 0; r < p.topk_group; ++r) {
+      last = rgk_wave_max(gk);
+      const int i = __builtin_ctzll(__ballot(gk == last)) >> w;
+      groups |= 1ull << i;
+      if (g == i) gk = 0;
+    }
+    if (gap > 0) {   // the best that is left may be as good as the last one taken (a sum is off by twice as much)
+      const K next = rgk_wave_max(gk);
+      if (!(rgk_value(last) - rgk_value(next) > (p.top2 ? 2 * gap : gap))) return false;
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int of = in_lanes ? g : (int)(((float)(e0 + j) + 0.5f) * p.inv_per);
+      if (j < n && !((groups >> of) & 1u)) key[j] = 0;
+    }
+  }
+  const bool gaps = std::is_same<V, float>::value && p.bias;
+  V before = 0;
+  for (int r = 0; r < p.topk; ++r) {
+    K k;
+    const int e = rgk_take<J>(key, &k);
+    if (lane == r) *mine = e;
+    if (gaps) {
+      const V now = rgk_value(k);
+      if (r && !(before - now > gap)) sure = false;
+      before = now;
+    }
+  }
+  if (gaps) {
+    K k = key[0];
+#pragma unroll
+    for (int j = 1; j < J; ++j) k = max(k, key[j]);
+    k = rgk_wave_max(k);
+    if (k && !(before - rgk_value(k) > gap)) sure = false;
+  }
+  return sure;
 }
 
 }  // namespace
 
+template <int J>
 __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(ZmiRouterGrouped p) {
-  __shared__ double value[RGK_WAVES][64 * RGK_PER_LANE];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  __shared__ double scratch[RGK_WAVES][64 * J];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int t = blockIdx.x * RGK_WAVES + wave;
   if (t >= p.T) return;   // (whole wavefronts; nothing below synchronizes across wavefronts)
-  float x[RGK_PER_LANE];
+  const int e0 = lane * J, n = p.E - e0;   // this lane's experts: e0 .. e0 + min(J, n) - 1
+  float x[J];
 #pragma unroll
-  for (int j = 0; j < RGK_PER_LANE; ++j) {
-    const int e = lane + 64 * j;
-    x[j] = e < p.E ? zmi_ld_f32(p.logits, p.logits_dt, (int64_t)t * p.ldl + e) : -__builtin_inff();
-  }
-  // ---- scores ----
-  double s[RGK_PER_LANE];
-  if (p.sigmoid) {
+  for (int j = 0; j < J; ++j) x[j] = -__builtin_inff();
+  const int64_t at = (int64_t)t * p.ldl + e0;
+  if (n >= J) {
+    if (p.logits_dt == ZMI_DT_F32) {
+      __builtin_memcpy(x, (const float *)p.logits + at, J * 4);
+    } else {
+      uint16_t h[J];
+      __builtin_memcpy(h, (const uint16_t *)p.logits + at, J * 2);
 #pragma unroll
-    for (int j = 0; j < RGK_PER_LANE; ++j) s[j] = 1.0 / (1.0 + exp(-(double)x[j]));
+      for (int j = 0; j < J; ++j) x[j] = p.logits_dt == ZMI_DT_BF16 ? zmi_bf16_to_f32(h[j]) : zmi_f16_to_f32(h[j]);
+    }
   } else {
-    float m = x[0];
 #pragma unroll
-    for (int j = 1; j < RGK_PER_LANE; ++j) m = fmaxf(m, x[j]);
+    for (int j = 0; j < J; ++j)
+      if (j < n) x[j] = zmi_ld_f32(p.logits, p.logits_dt, at + j);
+  }
+  uint32_t key[J];
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    double sum = 0.0;
+  for (int j = 0; j < J; ++j) key[j] = j < n ? rgk_key(x[j]) : 0u;
+  // ---- softmax: the row's maximum and sum ----
+  float m = 0.0f;
+  double sum = 0.0;
+  if (!p.sigmoid) {
+    uint32_t k = key[0];
 #pragma unroll
-    for (int j = 0; j < RGK_PER_LANE; ++j) {
-      // (a row's largest logit may be infinite: equal to the maximum is 1 whatever it is, -inf is 0)
-      s[j] = x[j] == -__builtin_inff() ? 0.0 : x[j] == m ? 1.0 : exp((double)x[j] - (double)m);
-      sum += s[j];
+    for (int j = 1; j < J; ++j) k = max(k, key[j]);
+    m = rgk_value(rgk_wave_max(k));
+#pragma unroll
+    // (equal to the maximum is 1, whatever it is, and -inf is 0; NaN stays)
+    for (int j = 0; j < J; ++j) sum += x[j] == -__builtin_inff() ? 0.0 : x[j] == m ? 1.0 : (double)zmi_expf(x[j] - m);
+    sum = rgk_wave_sum(sum);
+  }
+  bool sure = true;
+  float gap = 0.0f;   // values further apart than this are in their exact values' order
+  const bool valued = p.bias || (p.top2 && p.topk_group < p.n_group);
+  float v[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) v[j] = 0.0f;
+  if (valued) {
+    const float inv = p.sigmoid ? 0.0f : sum == 0.0 ? 0.0f : 1.0f / (float)sum;
+    float big = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      // (scores: at most 4 ulp off; the value's own rounding is half an ulp of it)
+      v[j] = p.sigmoid ? zmi_sigmoid(x[j]) : x[j] == -__builtin_inff() ? 0.0f : x[j] == m ? inv : zmi_expf(x[j] - m) * inv;
+      if (p.bias && j < n) v[j] += p.bias[e0 + j];
+      nan |= j < n && v[j] != v[j];
+      if (j < n && __builtin_fabsf(v[j]) < __builtin_inff()) big = fmaxf(big, __builtin_fabsf(v[j]));
+      if (p.bias) key[j] = j < n ? rgk_key(v[j]) : 0u;
     }
-    sum = rgk_sum(sum);
-#pragma unroll
-    for (int j = 0; j < RGK_PER_LANE; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] / sum;
+    sure = !__ballot(nan);
+    gap = 0x1p-19f * (p.sigmoid ? 1.0f : inv) + 0x1p-22f * __uint_as_float(rgk_wave_max(__float_as_uint(big)));
   }
-  // ---- values: without a bias the logits' own order ----
-  double v[RGK_PER_LANE];
-  uint64_t key[RGK_PER_LANE];
+  int mine = 0;
+  if (sure) sure = rgk_choose<J>(p, key, v, gap, scratch[wave], &mine);
+  if (!sure) {
+    double v64[J];
+    uint64_t key64[J];
 #pragma unroll
-  for (int j = 0; j < RGK_PER_LANE; ++j) {
-    const int e = lane + 64 * j;
-    v[j] = p.bias && e < p.E ? s[j] + (double)p.bias[e] : s[j];
-    key[j] = rgk_key(p.bias ? v[j] : (double)x[j]);
-  }
-  uint64_t groups = ~0ull;   // bit g: group g may be chosen from
-  const int per = p.E / p.n_group;
-  if (p.topk_group < p.n_group) {
-    const bool by_logit = !p.bias && !p.top2;
-#pragma unroll
-    for (int j = 0; j < RGK_PER_LANE; ++j)
-      if (lane + 64 * j < p.E) value[wave][lane + 64 * j] = by_logit ? (double)x[j] : v[j];
-    // (one wavefront writes and reads its own slice: the order of its LDS instructions is all that is needed)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    uint64_t gk = 0;
-    if (lane < p.n_group) {
-      double b1 = value[wave][lane * per], b2 = -__builtin_inf();
-      bool second = false;
-      for (int i = 1; i < per; ++i) {
-        const double a = value[wave][lane * per + i];
-        if (rgk_key(a) > rgk_key(b1)) { b2 = b1; b1 = a; }
-        else if (!second || rgk_key(a) > rgk_key(b2)) b2 = a;
-        second = true;
-      }
-      gk = rgk_key(p.top2 ? b1 + b2 : b1);
+    for (int j = 0; j < J; ++j) {
+      const double e = exp(p.sigmoid ? -(double)x[j] : (double)x[j] - (double)m);
+      v64[j] = p.sigmoid ? 1.0 / (1.0 + e) : x[j] == -__builtin_inff() || sum == 0.0 ? 0.0 : x[j] == m ? 1.0 : e;
     }
-    groups = 0;
-    for (int r = 0; r < p.topk_group; ++r) {
-      uint64_t k = gk;
-      int i = lane < p.n_group && !((groups >> lane) & 1u) ? lane : -1;
-      rgk_best(k, i);
-      groups |= 1ull << i;
+    if (!p.sigmoid) {
+      double z = 0.0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) z += v64[j];
+      z = rgk_wave_sum(z);
+#pragma unroll
+      for (int j = 0; j < J; ++j) v64[j] = z == 0.0 ? 0.0 : v64[j] / z;
     }
-  }
-  // ---- topk rounds ----
-  unsigned live = 0;
 #pragma unroll
-  for (int j = 0; j < RGK_PER_LANE; ++j) {
-    const int e = lane + 64 * j;
-    if (e < p.E && ((groups >> (e / per)) & 1u)) live |= 1u << j;
+    for (int j = 0; j < J; ++j) {
+      if (p.bias && j < n) v64[j] += (double)p.bias[e0 + j];
+      key64[j] = j >= n ? 0u : p.bias ? rgk_key(v64[j]) : rgk_key((double)x[j]);
+    }
+    rgk_choose<J>(p, key64, v64, 0.0, scratch[wave], &mine);
   }
-  double sel = 0.0, mine = 0.0;
-  for (int r = 0; r < p.topk; ++r) {
-    uint64_t k = 0;
-    int i = -1;
-    double sv = 0.0;
-#pragma unroll
-    for (int j = 0; j < RGK_PER_LANE; ++j)
-      if (((live >> j) & 1u) && (i < 0 || key[j] > k)) { k = key[j]; i = lane + 64 * j; sv = s[j]; }
-    rgk_best(k, i);
-    if (i % 64 == lane) live &= ~(1u << (i / 64));
-    sv = __shfl(sv, i % 64, 64);
-    sel += sv;
-    if (lane == r) mine = sv;
-    if (lane == 0) p.topk_ids[(int64_t)t * p.topk + r] = i;
+  // ---- weights: exponentials in f32, the rest in 64 bits ----
+  double s = 0.0;
+  if (lane < p.topk) {
+    const float y = zmi_ld_f32(p.logits, p.logits_dt, (int64_t)t * p.ldl + mine);
+    const float d = p.sigmoid ? -y : y - m;
+    // (scores near the end of f32's range count where all chosen are there)
+    const double e = __builtin_fabsf(d) < 80.0f ? (double)zmi_expf(d) : exp(p.sigmoid ? -(double)y : (double)y - (double)m);
+    s = p.sigmoid ? 1.0 / (1.0 + e) : y == -__builtin_inff() ? 0.0 : y == m ? 1.0 : e;
   }
-  if (p.renormalize) mine = sel == 0.0 ? 0.0 : mine / sel;
-  if (lane < p.topk) p.topk_weights[(int64_t)t * p.topk + lane] = (float)(mine * (double)p.scale);
+  const double z = p.renormalize ? rgk_wave_sum(s) : p.sigmoid ? 1.0 : sum;
+  if (lane < p.topk) {
+    p.topk_ids[(int64_t)t * p.topk + lane] = mine;
+    p.topk_weights[(int64_t)t * p.topk + lane] = z == 0.0 ? 0.0f : (float)(s / z * (double)p.scale);
+  }
 }
 
-hipError_t zmi_launch_moe_router_grouped(const ZmiRouterGrouped &p, hipStream_t stream) {
+hipError_t zmi_launch_moe_router_grouped(ZmiRouterGrouped p, hipStream_t stream) {
   if (p.T <= 0) return hipSuccess;
-  if (p.E <= 0 || p.E > 64 * RGK_PER_LANE || p.n_group <= 0 || p.n_group > 64 || p.E % p.n_group || p.topk_group <= 0 ||
+  if (p.E <= 0 || p.E > 512 || p.n_group <= 0 || p.n_group > 64 || p.E % p.n_group || p.topk_group <= 0 ||
       p.topk_group > p.n_group || p.topk <= 0 || p.topk > 64 || p.topk > p.topk_group * (p.E / p.n_group))
     return hipErrorInvalidValue;
-  hipLaunchKernelGGL(zmi_moe_router_grouped_kernel, dim3((unsigned)((p.T + RGK_WAVES - 1) / RGK_WAVES)), dim3(RGK_WAVES * 64), 0,
-                     stream, p);
+  // a group that fills 1, 2, 4, 8 or 16 whole lanes is valued in registers, others through LDS
+  const int J = p.E <= 64 ? 1 : p.E <= 128 ? 2 : p.E <= 256 ? 4 : 8, lanes = p.E / p.n_group / J;
+  p.per = p.E / p.n_group;
+  p.inv_per = 1.0f / (float)p.per;   // (e + 0.5) times it truncates to e / per for every e < 512
+  p.lane_shift = p.per % J == 0 && lanes <= 16 && (lanes & (lanes - 1)) == 0 ? __builtin_ctz(lanes) : -1;
+  const dim3 grid((unsigned)((p.T + RGK_WAVES - 1) / RGK_WAVES)), block(RGK_WAVES * 64);
+  if (J == 1) hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<1>, grid, block, 0, stream, p);
+  else if (J == 2) hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<2>, grid, block, 0, stream, p);
+  else if (J == 4) hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<4>, grid, block, 0, stream, p);
+  else hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<8>, grid, block, 0, stream, p);
   return hipGetLastError();
 }

@@ -869,7 +869,7 @@ int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r) {
   }
   note_operand(r->logits); note_operand(r->bias); note_operand(r->topk_ids); note_operand(r->topk_weights);
   if (!ensure_device()) return ZMI_FAILURE;
-  ZmiRouterGrouped p;
+  ZmiRouterGrouped p = {};
   p.logits = r->logits; p.ldl = r->ldl; p.bias = r->bias; p.topk_ids = r->topk_ids; p.topk_weights = r->topk_weights;
   p.logits_dt = r->logits_dt; p.T = r->T; p.E = r->E; p.topk = r->topk; p.n_group = r->n_group; p.topk_group = r->topk_group;
   p.sigmoid = r->scoring == ZMI_SCORE_SIGMOID; p.top2 = r->group_score == ZMI_GROUP_TOP2_SUM;

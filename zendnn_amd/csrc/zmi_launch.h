@@ -321,8 +321,10 @@ struct ZmiRouterGrouped {
   int32_t top2;               // 1: a group's value is the sum of its two best
   int32_t renormalize;
   float scale;
+  int32_t per, lane_shift;    // (the launcher's own: experts of a group, log2 of the lanes it fills)
+  float inv_per;
 };
-hipError_t zmi_launch_moe_router_grouped(const ZmiRouterGrouped &p, hipStream_t stream);
+hipError_t zmi_launch_moe_router_grouped(ZmiRouterGrouped p, hipStream_t stream);
 
 // k_lora.hip: zmi_lora_t with its rules checked (the operands' meaning is described there)
 struct ZmiLora {
