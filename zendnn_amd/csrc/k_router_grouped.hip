@@ -70,29 +70,28 @@ __device__ __forceinline__ uint64_t rgk_key(double x) {
 __device__ __forceinline__ float rgk_value(uint32_t k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ double rgk_value(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k)); }
 
-// One round over the wavefront's J keys a lane: the largest key's first holder (lowest lane, then lowest j) is taken out;
-// returns its expert and, in *best, the key.
+// A lane's J keys in descending order, equal ones in ascending j (neighbours are exchanged only when out of order);
+// returns the j of each, four bits apiece, the first in the lowest bits.
 template <int J, class K>
-__device__ __forceinline__ int rgk_take(K (&key)[J], K *best) {
-  K m = key[0];
+__device__ __forceinline__ uint32_t rgk_sort(K (&key)[J]) {
+  // (a vector, not an array: choosing between two elements of an array becomes an indexed read, a chain of comparisons)
+  typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+  u32x8 at = {0, 1, 2, 3, 4, 5, 6, 7};
+  uint32_t queue = 0;
 #pragma unroll
-  for (int j = 1; j < J; ++j) m = max(m, key[j]);
-  const K top = rgk_wave_max(m);
-  uint64_t hit[J], any = 0;
+  for (int r = 0; r < J; ++r)
 #pragma unroll
-  for (int j = 0; j < J; ++j) { hit[j] = __ballot(key[j] == top); any |= hit[j]; }
-  const int lane = __builtin_ctzll(any);
-  uint64_t open = 1ull << lane;
-  int at = 0;
+    for (int j = r % 2; j + 1 < J; j += 2) {
+      const bool swap = key[j + 1] > key[j];
+      const K hi = max(key[j], key[j + 1]), lo = min(key[j], key[j + 1]);
+      const uint32_t a = at[j], b = at[j + 1];
+      key[j] = hi; key[j + 1] = lo;
+      at[j] = swap ? b : a;
+      at[j + 1] = swap ? a : b;
+    }
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const uint64_t mine = hit[j] & open;
-    if (mine) at = j;
-    open &= ~mine;
-    if ((threadIdx.x % 64) == lane && mine) key[j] = 0;
-  }
-  *best = top;
-  return lane * J + at;
+  for (int j = 0; j < J; ++j) queue |= at[j] << (4 * j);
+  return queue;
 }
 
 // The two largest of two lanes, from the two largest of each.
@@ -159,114 +158,141 @@ __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J
       if (j < n && !((groups >> of) & 1u)) key[j] = 0;
     }
   }
-  const bool gaps = std::is_same<V, float>::value && p.bias;
-  V before = 0;
+  // rounds: the largest first key of a lane, of the lowest lane that has it
+  uint32_t queue = rgk_sort<J>(key);
+  uint32_t order = 0;   // float values: lane r keeps the r-th key
   for (int r = 0; r < p.topk; ++r) {
-    K k;
-    const int e = rgk_take<J>(key, &k);
-    if (lane == r) *mine = e;
-    if (gaps) {
-      const V now = rgk_value(k);
-      if (r && !(before - now > gap)) sure = false;
-      before = now;
+    const K top = rgk_wave_max(key[0]);
+    const int at = __builtin_ctzll(__ballot(key[0] == top));
+    const int e = at * J + (__builtin_amdgcn_readlane((int)queue, at) & 15);
+    if (lane == r) { *mine = e; order = (uint32_t)top; }
+    if (lane == at) {
+#pragma unroll
+      for (int j = 0; j + 1 < J; ++j) key[j] = key[j + 1];
+      key[J - 1] = 0;
+      queue >>= 4;
     }
   }
-  if (gaps) {
-    K k = key[0];
-#pragma unroll
-    for (int j = 1; j < J; ++j) k = max(k, key[j]);
-    k = rgk_wave_max(k);
-    if (k && !(before - rgk_value(k) > gap)) sure = false;
+  if (std::is_same<V, float>::value && p.bias) {
+    const uint32_t rest = (uint32_t)rgk_wave_max(key[0]), below = (uint32_t)__shfl_down((int)order, 1, 64);
+    const uint32_t next = lane == p.topk - 1 ? rest : below;
+    const bool close = lane < p.topk && next && !(rgk_value(order) - rgk_value(next) > (float)gap);
+    if (__ballot(close)) sure = false;
   }
   return sure;
 }
 
 }  // namespace
 
-template <int J>
+template <int J, bool SIGMOID>
 __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(ZmiRouterGrouped p) {
   __shared__ double scratch[RGK_WAVES][64 * J];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int t = blockIdx.x * RGK_WAVES + wave;
   if (t >= p.T) return;   // (whole wavefronts; nothing below synchronizes across wavefronts)
   const int e0 = lane * J, n = p.E - e0;   // this lane's experts: e0 .. e0 + min(J, n) - 1
-  float x[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) x[j] = -__builtin_inff();
-  const int64_t at = (int64_t)t * p.ldl + e0;
-  if (n >= J) {
-    if (p.logits_dt == ZMI_DT_F32) {
-      __builtin_memcpy(x, (const float *)p.logits + at, J * 4);
+  const int64_t row = (int64_t)t * p.ldl;
+  float x[J], bias[J];
+  // (lanes at the end read the last expert's word in the place of what is not there)
+  if (p.logits_dt == ZMI_DT_F32) {
+    const float *f = (const float *)p.logits + row;
+    if (n >= J) {
+      __builtin_memcpy(x, f + e0, J * 4);
     } else {
-      uint16_t h[J];
-      __builtin_memcpy(h, (const uint16_t *)p.logits + at, J * 2);
 #pragma unroll
-      for (int j = 0; j < J; ++j) x[j] = p.logits_dt == ZMI_DT_BF16 ? zmi_bf16_to_f32(h[j]) : zmi_f16_to_f32(h[j]);
+      for (int j = 0; j < J; ++j) x[j] = f[j < n ? e0 + j : p.E - 1];
     }
   } else {
+    const uint16_t *f = (const uint16_t *)p.logits + row;
+    uint16_t h[J];
+    if (n >= J) {
+      __builtin_memcpy(h, f + e0, J * 2);
+    } else {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (j < n) x[j] = zmi_ld_f32(p.logits, p.logits_dt, at + j);
+      for (int j = 0; j < J; ++j) h[j] = f[j < n ? e0 + j : p.E - 1];
+    }
+    const bool bf16 = p.logits_dt == ZMI_DT_BF16;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const float a = zmi_bf16_to_f32(h[j]), b = zmi_f16_to_f32(h[j]);
+      x[j] = bf16 ? a : b;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) bias[j] = 0.0f;
+  if (p.bias) {
+    if (n >= J) {
+      __builtin_memcpy(bias, p.bias + e0, J * 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j) bias[j] = p.bias[j < n ? e0 + j : p.E - 1];
+    }
   }
   uint32_t key[J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) key[j] = j < n ? rgk_key(x[j]) : 0u;
+  for (int j = 0; j < J; ++j) {
+    if (j >= n) x[j] = -__builtin_inff();
+    key[j] = j < n ? rgk_key(x[j]) : 0u;
+  }
   // ---- softmax: the row's maximum and sum ----
-  float m = 0.0f;
+  float m = 0.0f, v[J];
   double sum = 0.0;
-  if (!p.sigmoid) {
+  if (!SIGMOID) {
     uint32_t k = key[0];
 #pragma unroll
     for (int j = 1; j < J; ++j) k = max(k, key[j]);
     m = rgk_value(rgk_wave_max(k));
+    float part[J];
 #pragma unroll
-    // (equal to the maximum is 1, whatever it is, and -inf is 0; NaN stays)
-    for (int j = 0; j < J; ++j) sum += x[j] == -__builtin_inff() ? 0.0 : x[j] == m ? 1.0 : (double)zmi_expf(x[j] - m);
-    sum = rgk_wave_sum(sum);
+    for (int j = 0; j < J; ++j) {
+      // (equal to the maximum is 1, whatever it is, and -inf is 0; NaN stays)
+      v[j] = zmi_expf(x[j] - m);
+      v[j] = x[j] == m ? 1.0f : v[j];
+      v[j] = x[j] == -__builtin_inff() ? 0.0f : v[j];
+      part[j] = v[j];
+    }
+    // (a lane's terms are added in f32, at most three roundings deep, the lanes' sums in 64 bits)
+#pragma unroll
+    for (int w = J / 2; w >= 1; w /= 2)
+#pragma unroll
+      for (int j = 0; j < w; ++j) part[j] += part[j + w];
+    sum = rgk_wave_sum((double)part[0]);
   }
   bool sure = true;
   float gap = 0.0f;   // values further apart than this are in their exact values' order
-  const bool valued = p.bias || (p.top2 && p.topk_group < p.n_group);
-  float v[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) v[j] = 0.0f;
-  if (valued) {
-    const float inv = p.sigmoid ? 0.0f : sum == 0.0 ? 0.0f : 1.0f / (float)sum;
-    float big = 0.0f;
+  if (p.bias || (p.top2 && p.topk_group < p.n_group)) {
+    const float top = SIGMOID ? 1.0f : sum == 0.0 ? 0.0f : 1.0f / (float)sum;
+    uint32_t big = 0;
     bool nan = false;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       // (scores: at most 4 ulp off; the value's own rounding is half an ulp of it)
-      v[j] = p.sigmoid ? zmi_sigmoid(x[j]) : x[j] == -__builtin_inff() ? 0.0f : x[j] == m ? inv : zmi_expf(x[j] - m) * inv;
-      if (p.bias && j < n) v[j] += p.bias[e0 + j];
-      nan |= j < n && v[j] != v[j];
-      if (j < n && __builtin_fabsf(v[j]) < __builtin_inff()) big = fmaxf(big, __builtin_fabsf(v[j]));
+      v[j] = (SIGMOID ? zmi_sigmoid(x[j]) : v[j] * top) + bias[j];
+      const uint32_t size = __float_as_uint(v[j]) & 0x7fffffffu;
+      nan |= j < n && size > 0x7f800000u;
+      big = max(big, j < n && size < 0x7f800000u ? size : 0u);
       if (p.bias) key[j] = j < n ? rgk_key(v[j]) : 0u;
     }
     sure = !__ballot(nan);
-    gap = 0x1p-19f * (p.sigmoid ? 1.0f : inv) + 0x1p-22f * __uint_as_float(rgk_wave_max(__float_as_uint(big)));
+    gap = 0x1p-19f * top + 0x1p-22f * __uint_as_float(rgk_wave_max(big));
   }
   int mine = 0;
   if (sure) sure = rgk_choose<J>(p, key, v, gap, scratch[wave], &mine);
   if (!sure) {
     double v64[J];
     uint64_t key64[J];
+    double z = 0.0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const double e = exp(p.sigmoid ? -(double)x[j] : (double)x[j] - (double)m);
-      v64[j] = p.sigmoid ? 1.0 / (1.0 + e) : x[j] == -__builtin_inff() || sum == 0.0 ? 0.0 : x[j] == m ? 1.0 : e;
+      const double e = exp(SIGMOID ? -(double)x[j] : (double)x[j] - (double)m);
+      v64[j] = SIGMOID ? 1.0 / (1.0 + e) : x[j] == -__builtin_inff() ? 0.0 : x[j] == m ? 1.0 : e;
+      z += v64[j];
     }
-    if (!p.sigmoid) {
-      double z = 0.0;
-#pragma unroll
-      for (int j = 0; j < J; ++j) z += v64[j];
-      z = rgk_wave_sum(z);
-#pragma unroll
-      for (int j = 0; j < J; ++j) v64[j] = z == 0.0 ? 0.0 : v64[j] / z;
-    }
+    if (!SIGMOID) z = rgk_wave_sum(z);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (p.bias && j < n) v64[j] += (double)p.bias[e0 + j];
+      if (!SIGMOID) v64[j] = z == 0.0 ? 0.0 : v64[j] / z;
+      v64[j] += (double)bias[j];
       key64[j] = j >= n ? 0u : p.bias ? rgk_key(v64[j]) : rgk_key((double)x[j]);
     }
     rgk_choose<J>(p, key64, v64, 0.0, scratch[wave], &mine);
@@ -274,18 +300,29 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
   // ---- weights: exponentials in f32, the rest in 64 bits ----
   double s = 0.0;
   if (lane < p.topk) {
-    const float y = zmi_ld_f32(p.logits, p.logits_dt, (int64_t)t * p.ldl + mine);
-    const float d = p.sigmoid ? -y : y - m;
+    const float y = zmi_ld_f32(p.logits, p.logits_dt, row + mine), d = SIGMOID ? -y : y - m;
+    double e = (double)zmi_expf(d);
     // (scores near the end of f32's range count where all chosen are there)
-    const double e = __builtin_fabsf(d) < 80.0f ? (double)zmi_expf(d) : exp(p.sigmoid ? -(double)y : (double)y - (double)m);
-    s = p.sigmoid ? 1.0 / (1.0 + e) : y == -__builtin_inff() ? 0.0 : y == m ? 1.0 : e;
+    if (__builtin_fabsf(d) >= 80.0f) e = exp(SIGMOID ? -(double)y : (double)y - (double)m);
+    s = SIGMOID ? 1.0 / (1.0 + e) : y == -__builtin_inff() ? 0.0 : y == m ? 1.0 : e;
   }
-  const double z = p.renormalize ? rgk_wave_sum(s) : p.sigmoid ? 1.0 : sum;
+  const double z = p.renormalize ? rgk_wave_sum(s) : SIGMOID ? 1.0 : sum;
   if (lane < p.topk) {
     p.topk_ids[(int64_t)t * p.topk + lane] = mine;
     p.topk_weights[(int64_t)t * p.topk + lane] = z == 0.0 ? 0.0f : (float)(s / z * (double)p.scale);
   }
 }
+
+namespace {
+
+template <int J>
+void rgk_launch(const ZmiRouterGrouped &p, hipStream_t stream) {
+  const dim3 grid((unsigned)((p.T + RGK_WAVES - 1) / RGK_WAVES)), block(RGK_WAVES * 64);
+  if (p.sigmoid) hipLaunchKernelGGL((zmi_moe_router_grouped_kernel<J, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((zmi_moe_router_grouped_kernel<J, false>), grid, block, 0, stream, p);
+}
+
+}  // namespace
 
 hipError_t zmi_launch_moe_router_grouped(ZmiRouterGrouped p, hipStream_t stream) {
   if (p.T <= 0) return hipSuccess;
@@ -297,10 +334,9 @@ hipError_t zmi_launch_moe_router_grouped(ZmiRouterGrouped p, hipStream_t stream)
   p.per = p.E / p.n_group;
   p.inv_per = 1.0f / (float)p.per;   // (e + 0.5) times it truncates to e / per for every e < 512
   p.lane_shift = p.per % J == 0 && lanes <= 16 && (lanes & (lanes - 1)) == 0 ? __builtin_ctz(lanes) : -1;
-  const dim3 grid((unsigned)((p.T + RGK_WAVES - 1) / RGK_WAVES)), block(RGK_WAVES * 64);
-  if (J == 1) hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<1>, grid, block, 0, stream, p);
-  else if (J == 2) hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<2>, grid, block, 0, stream, p);
-  else if (J == 4) hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<4>, grid, block, 0, stream, p);
-  else hipLaunchKernelGGL(zmi_moe_router_grouped_kernel<8>, grid, block, 0, stream, p);
+  if (J == 1) rgk_launch<1>(p, stream);
+  else if (J == 2) rgk_launch<2>(p, stream);
+  else if (J == 4) rgk_launch<4>(p, stream);
+  else rgk_launch<8>(p, stream);
   return hipGetLastError();
 }
