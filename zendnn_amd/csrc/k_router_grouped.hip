@@ -58,6 +58,16 @@ __device__ __forceinline__ double rgk_wave_sum(double v) {
                                           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), 63) << 32));
 }
 
+// exp(d) for d <= 0 (NaN stays), as zmi_expf without what only overflow needs; 0 below -200
+__device__ __forceinline__ float rgk_exp_down(float d) {
+  const float l2e_hi = 1.44269502162933349609375f, l2e_lo = 1.925963033500011e-08f;
+  d = d < -200.0f ? -200.0f : d;   // (infinities would meet in the correction)
+  const float t = d * l2e_hi;
+  const float r = __builtin_fmaf(d, l2e_lo, __builtin_fmaf(d, l2e_hi, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, r * 0.693147182464599609375f, e);
+}
+
 // value -> unsigned key in the values' order; -0 == +0; NaN 1, below every number (0: nothing)
 __device__ __forceinline__ uint32_t rgk_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
@@ -102,12 +112,15 @@ __device__ __forceinline__ void rgk_pair(K &a, K &b) {
   a = max(a, c);
 }
 
-// The choice.  key: what experts are ordered by, v: the values that groups are valued by (top2); both of V's type.  V
-// float: false when a gap that decides is not above `gap`.  Lane r gets the r-th expert.
+// The choice.  key: what experts are ordered by, v: the values that groups are valued by (top2); both of V's type.  Lane r
+// gets the r-th expert.
+//
+// Float keys (with a bias) and v are f32 values of scores up to `score`: false when a gap that decides is not wide enough.  A score is at most 4 ulp off, 2^-21 score, and rounding a value adds half an ulp of it, so two values that
+// lie 2^-20 score + 2^-24 (|a| + |b|) apart are in the order of the exact ones; twice that is asked for.  Values below the
+// one compared with can be off by more where they are larger, but then they are negative and far below.
 template <int J, class V, class K>
-__device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J], const V (&v)[J], V gap, void *scratch, int *mine) {
+__device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J], const V (&v)[J], float score, void *scratch, int *mine) {
   const int lane = threadIdx.x % 64, e0 = lane * J, n = p.E - e0, per = p.per;
-  bool sure = true;
   if (p.topk_group < p.n_group) {
     K a = 0, b = 0;   // a lane's, then its group's, two largest
     const bool in_lanes = p.lane_shift >= 0;
@@ -148,9 +161,13 @@ __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J
       groups |= 1ull << i;
       if (g == i) gk = 0;
     }
-    if (gap > 0) {   // the best that is left may be as good as the last one taken (a sum is off by twice as much)
-      const K next = rgk_wave_max(gk);
-      if (!(rgk_value(last) - rgk_value(next) > (p.top2 ? 2 * gap : gap))) return false;
+    if (std::is_same<V, float>::value && (p.bias || p.top2)) {
+      // the best that is left may be as good as the last one taken (a sum is off by twice as much, and by its rounding)
+      const float next = (float)rgk_value(rgk_wave_max(gk)), taken = (float)rgk_value(last);
+      float size = __builtin_fabsf((float)rgk_value(a)) + (p.top2 ? __builtin_fabsf((float)rgk_value(b)) : 0.0f);
+      if (g >= p.n_group || !(size < __builtin_inff())) size = 0.0f;
+      size = __uint_as_float(rgk_wave_max(__float_as_uint(size)));
+      if (!(taken - next > 0x1p-18f * score + 0x1p-21f * size)) return false;
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -176,10 +193,11 @@ __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J
   if (std::is_same<V, float>::value && p.bias) {
     const uint32_t rest = (uint32_t)rgk_wave_max(key[0]), below = (uint32_t)__shfl_down((int)order, 1, 64);
     const uint32_t next = lane == p.topk - 1 ? rest : below;
-    const bool close = lane < p.topk && next && !(rgk_value(order) - rgk_value(next) > (float)gap);
-    if (__ballot(close)) sure = false;
+    const float a = rgk_value(order), b = rgk_value(next);
+    const bool close = lane < p.topk && next && !(a - b > 0x1p-19f * score + 0x1p-23f * (__builtin_fabsf(a) + __builtin_fabsf(b)));
+    if (__ballot(close)) return false;
   }
-  return sure;
+  return true;
 }
 
 }  // namespace
@@ -230,23 +248,21 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
   }
   uint32_t key[J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
+  for (int j = 0; j < J; ++j)
     if (j >= n) x[j] = -__builtin_inff();
-    key[j] = j < n ? rgk_key(x[j]) : 0u;
-  }
   // ---- softmax: the row's maximum and sum ----
   float m = 0.0f, v[J];
   double sum = 0.0;
   if (!SIGMOID) {
-    uint32_t k = key[0];
+    float top = x[0];
 #pragma unroll
-    for (int j = 1; j < J; ++j) k = max(k, key[j]);
-    m = rgk_value(rgk_wave_max(k));
+    for (int j = 1; j < J; ++j) top = fmaxf(top, x[j]);   // (skips NaN; a NaN logit reaches the sum below)
+    m = rgk_value(rgk_wave_max(rgk_key(top)));
     float part[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       // (equal to the maximum is 1, whatever it is, and -inf is 0; NaN stays)
-      v[j] = zmi_expf(x[j] - m);
+      v[j] = rgk_exp_down(x[j] - m);
       v[j] = x[j] == m ? 1.0f : v[j];
       v[j] = x[j] == -__builtin_inff() ? 0.0f : v[j];
       part[j] = v[j];
@@ -258,27 +274,22 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
       for (int j = 0; j < w; ++j) part[j] += part[j + w];
     sum = rgk_wave_sum((double)part[0]);
   }
-  bool sure = true;
-  float gap = 0.0f;   // values further apart than this are in their exact values' order
+  float score = 0.0f;   // the largest score there can be, where values are f32 scores
   if (p.bias || (p.top2 && p.topk_group < p.n_group)) {
     const float top = SIGMOID ? 1.0f : sum == 0.0 ? 0.0f : 1.0f / (float)sum;
-    uint32_t big = 0;
-    bool nan = false;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      // (scores: at most 4 ulp off; the value's own rounding is half an ulp of it)
       v[j] = (SIGMOID ? zmi_sigmoid(x[j]) : v[j] * top) + bias[j];
-      const uint32_t size = __float_as_uint(v[j]) & 0x7fffffffu;
-      nan |= j < n && size > 0x7f800000u;
-      big = max(big, j < n && size < 0x7f800000u ? size : 0u);
       if (p.bias) key[j] = j < n ? rgk_key(v[j]) : 0u;
     }
-    sure = !__ballot(nan);
-    gap = 0x1p-19f * top + 0x1p-22f * __uint_as_float(rgk_wave_max(big));
+    score = top;
+  }
+  if (!p.bias) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) key[j] = j < n ? rgk_key(x[j]) : 0u;
   }
   int mine = 0;
-  if (sure) sure = rgk_choose<J>(p, key, v, gap, scratch[wave], &mine);
-  if (!sure) {
+  if (!rgk_choose<J>(p, key, v, score, scratch[wave], &mine)) {
     double v64[J];
     uint64_t key64[J];
     double z = 0.0;
@@ -295,7 +306,7 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
       v64[j] += (double)bias[j];
       key64[j] = j >= n ? 0u : p.bias ? rgk_key(v64[j]) : rgk_key((double)x[j]);
     }
-    rgk_choose<J>(p, key64, v64, 0.0, scratch[wave], &mine);
+    rgk_choose<J>(p, key64, v64, 0.0f, scratch[wave], &mine);
   }
   // ---- weights: exponentials in f32, the rest in 64 bits ----
   double s = 0.0;
