@@ -8,10 +8,8 @@
 //
 //   plan    (more than 64 rows) one workgroup sorts the rows by slot and lists the tiles; up to 64 rows every
 //           wavefront finds its tile by itself from a ballot per distinct id, and there is no such launch;
-//   shrink  h of a tile.  Wavefronts split K, not the tile: operands go straight from memory to registers, each
-//           wavefront has its own loads in flight and no barrier in its loop; partial sums meet in LDS, and across
-//           the workgroups of one tile (K in slices, where the tiles alone do not fill the device) in memory;
-//   expand  dst.  A wavefront takes 64 columns of a tile's rows and reads h as MFMA operands.
+//   shrink  h of a tile, K through an LDS ring.  K is cut into slices where the tiles alone do not fill the device;
+//   expand  dst.  A wavefront keeps 32 .. 128 columns' B in registers and goes down the rows of its slot.
 //
 // The MFMA takes 16-bit operands: x, A exactly as they are; h, which is f32, as a sum of bf16 terms (2 terms hold 16
 // bits, for f32 destinations 3 hold 24), and f16 B, which the range of h does not allow to meet in f16, as two bf16 terms
@@ -23,7 +21,6 @@
 
 #define LORA_WAVES 4
 #define LORA_SMALL_T 64     // rows up to which wavefronts plan for themselves
-#define LORA_COLS 256       // columns of an expand workgroup
 
 namespace {
 
@@ -58,6 +55,7 @@ struct Tile {
   int n;      // rows of the tile
   int first;  // planned: position of its first row in the sorted order
   int row;    // unplanned: lane l's row is that of position l % 16
+  int group;  // planned: number of its first 16-row group in h
 };
 
 // Tile `want` of up to 64 rows: slots in the order of their first rows, 16 rows each.
@@ -92,12 +90,13 @@ __device__ __forceinline__ bool lora_find_tile(const ZmiLora &p, int want, Tile 
   return false;
 }
 
-__device__ __forceinline__ bool lora_planned_tile(const ZmiLoraPlan &w, int want, Tile &t) {
-  if (want >= w.header[0]) return false;
-  const int *e = w.tiles + 4 * (int64_t)want;
+__device__ __forceinline__ bool lora_planned_tile(const int32_t *table, int count, int want, Tile &t) {
+  if (want >= count) return false;
+  const int *e = table + 4 * (int64_t)want;
   t.slot = __builtin_amdgcn_readfirstlane(e[0]);
   t.first = __builtin_amdgcn_readfirstlane(e[1]);
   t.n = __builtin_amdgcn_readfirstlane(e[2]);
+  t.group = __builtin_amdgcn_readfirstlane(e[3]);
   t.row = 0;
   return true;
 }
@@ -123,150 +122,240 @@ __device__ __forceinline__ void split(const float (&v)[N], __bf16 (&t)[TERMS][N]
   }
 }
 
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// (LDS reads of the step before are over when a wavefront arrives: what follows may write where it read)
+__device__ __forceinline__ void group_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+extern __shared__ __attribute__((aligned(16))) char lora_smem[];
+
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------------------------
 // plan: rows sorted by slot (the order within a slot does not matter: rows are computed independently of each other),
-// tiles of at most `tile` rows.
+// the shrink launch's tiles of `tile` rows and the expand launch's, of `wide` times as many.
 // ---------------------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraPlan w, int tile) {
-  __shared__ int cursor[ZMI_LORA_MAX_SLOTS + 1];
-  __shared__ int wave_rows[16], wave_tiles[16];
+#define LORA_PLAN_KEEP 8   // ids a thread keeps between the passes
+
+__global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraPlan w, int tile, int wide) {
+  __shared__ int count[ZMI_LORA_MAX_SLOTS + 1];
+  __shared__ int wave_sums[3][16];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = p.n_slots + 1;
-  for (int i = tid; i < n; i += 1024) cursor[i] = 0;
-  for (int i = tid; i < w.n_arrivals; i += 1024) w.arrivals[i] = 0;
-  __syncthreads();
   auto slot_of = [&](int t) {
+    if (t >= p.T) return -1;
     const int id = p.slot_ids[t];
     return (unsigned)id < (unsigned)p.n_slots ? id : p.n_slots;
   };
-  for (int t = tid; t < p.T; t += 1024) atomicAdd(&cursor[slot_of(t)], 1);
+  int id[LORA_PLAN_KEEP], pos[LORA_PLAN_KEEP];
+#pragma unroll
+  for (int i = 0; i < LORA_PLAN_KEEP; ++i) id[i] = slot_of(i * 1024 + tid);
+  for (int i = tid; i < n; i += 1024) count[i] = 0;
+  for (int i = tid; i < w.n_arrivals; i += 1024) w.arrivals[i] = 0;
+  __syncthreads();
+  // a row's place among its slot's rows: rows of a wavefront that share a slot take their places with one atomic (the
+  // first few distinct slots; neighbouring rows mostly belong to one request)
+  auto place = [&](int mine) {
+    int at = 0;
+    bool open = mine >= 0;
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t left = __ballot(open);
+      if (!left) return at;
+      const int first = __builtin_ctzll(left), slot = __builtin_amdgcn_readlane(mine, first);
+      const uint64_t same = __ballot(open && mine == slot);
+      int base = 0;
+      if (lane == first) base = atomicAdd(&count[slot], (int)__popcll(same));
+      base = __builtin_amdgcn_readlane(base, first);
+      if (open && mine == slot) { at = base + __popcll(same & ((1ull << lane) - 1)); open = false; }
+    }
+    if (open) at = atomicAdd(&count[mine], 1);
+    return at;
+  };
+#pragma unroll
+  for (int i = 0; i < LORA_PLAN_KEEP; ++i)
+    if (i * 1024 < p.T) pos[i] = place(id[i]);
+  for (int t0 = LORA_PLAN_KEEP * 1024; t0 < p.T; t0 += 1024) {
+    const int at = place(slot_of(t0 + tid));
+    if (t0 + tid < p.T) w.place[t0 + tid] = at;
+  }
   __syncthreads();
   // thread i owns slots [i per, (i + 1) per)
   const int per = (n + 1023) / 1024;
-  int rows = 0, tiles = 0;
+  int sums[3] = {0, 0, 0};   // rows, tiles, wide tiles
   for (int i = tid * per; i < (tid + 1) * per && i < n; ++i) {
-    rows += cursor[i];
-    tiles += (cursor[i] + tile - 1) / tile;
+    const int c = count[i];
+    sums[0] += c;
+    sums[1] += (c + tile - 1) / tile;
+    sums[2] += (c + tile * wide - 1) / (tile * wide);
   }
-  int r = rows, q = tiles;
+  int start[3];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int a = __shfl_up(r, d, 64), b = __shfl_up(q, d, 64);
-    if (lane >= d) { r += a; q += b; }
-  }
-  if (lane == 63) { wave_rows[wave] = r; wave_tiles[wave] = q; }
-  __syncthreads();
-  int row0 = r - rows, tile0 = q - tiles;
-  for (int i = 0; i < wave; ++i) { row0 += wave_rows[i]; tile0 += wave_tiles[i]; }
-  if (tid == 1023) w.header[0] = tile0 + tiles;
-  for (int i = tid * per; i < (tid + 1) * per && i < n; ++i) {
-    const int c = cursor[i];
-    for (int j = 0; j < c; j += tile) {
-      int *e = w.tiles + 4 * (int64_t)tile0++;
-      e[0] = i;
-      e[1] = row0 + j;
-      e[2] = c - j < tile ? c - j : tile;
+  for (int k = 0; k < 3; ++k) {
+    int v = sums[k];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(v, d, 64);
+      if (lane >= d) v += o;
     }
-    cursor[i] = row0;
-    row0 += c;
+    if (lane == 63) wave_sums[k][wave] = v;
+    start[k] = v - sums[k];
   }
   __syncthreads();
-  for (int t = tid; t < p.T; t += 1024) w.order[atomicAdd(&cursor[slot_of(t)], 1)] = t;
+  for (int i = 0; i < wave; ++i)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) start[k] += wave_sums[k][i];
+  if (tid == 1023) {
+    w.header[0] = start[1] + sums[1];
+    w.header[1] = start[2] + sums[2];
+  }
+  for (int i = tid * per; i < (tid + 1) * per && i < n; ++i) {
+    const int c = count[i], tile0 = start[1];
+    for (int j = 0; j < c; j += tile)
+      *(int4 *)(w.tiles + 4 * (int64_t)start[1]++) = make_int4(i, start[0] + j, c - j < tile ? c - j : tile, (tile0 + j / tile) * (tile / 16));
+    for (int j = 0; j < c; j += tile * wide)
+      *(int4 *)(w.wide + 4 * (int64_t)start[2]++) = make_int4(i, start[0] + j, c - j < tile * wide ? c - j : tile * wide, (tile0 + j / tile) * (tile / 16));
+    count[i] = start[0];
+    start[0] += c;
+  }
+  __syncthreads();
+  // (each thread reads back the places that it wrote itself)
+  for (int t = LORA_PLAN_KEEP * 1024 + tid; t < p.T; t += 1024) w.order[count[slot_of(t)] + w.place[t]] = t;
+#pragma unroll
+  for (int i = 0; i < LORA_PLAN_KEEP; ++i)
+    if (id[i] >= 0) w.order[count[id[i]] + pos[i]] = i * 1024 + tid;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // shrink: workgroup (x: tile, y: NT rank tiles of 16, z: K slice).  MFMA rows are ranks, columns the tile's rows: lane
 // l holds ranks (l / 16) * 4 .. +3 of row l % 16.  Rank tiles are numbered over the live ones of all slices (an adapter
 // of a smaller rank has fewer); ranks and rows beyond the last one repeat it and are dropped.
+//
+// K goes through an LDS ring of D stages of KS elements: x rows and A rows alike are moved in units of 8 rows x 128
+// bytes, one 16-byte piece a lane.  (MFMA operands read from global memory directly put 16 rows under 16 neighbouring
+// lanes: every 16 bytes a cache line of its own, and the compute unit's address path, not HBM, sets the pace: 148 us for
+// 8192 rows of K = 14336 at rank 128 against 62 us through LDS.)  Piece c of row r stands at slot c ^ (r % 8), which
+// spreads the operand reads over the banks.  With rows, strides and addresses of 16-byte multiples the units are moved
+// by global -> LDS loads (DMA), D - 1 stages ahead; otherwise through registers, one stage ahead.
+// The four wavefronts share a stage as WR x WN x WK over row groups, rank tiles and 64-element blocks of K.
 // ---------------------------------------------------------------------------------------------------------------
-template <bool F16, int RT, int NT, int DEPTH, bool SMALL>
-__global__ __launch_bounds__(LORA_WAVES * 64, RT * NT < 32 ? 2 : 1) void zmi_lora_shrink_kernel(ZmiLora p, ZmiLoraPlan w) {
-  constexpr int FRAGS = RT * NT;
-  constexpr int PART = FRAGS < 8 ? FRAGS : 8;   // fragments summed over the wavefronts at a time
-  __shared__ f32x4 red[LORA_WAVES][PART][64];
-  __shared__ int is_last;
+template <bool F16, int RT, int NT, int KS, int WR, int WN, int D, bool DMA, bool SMALL>
+__global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(ZmiLora p, ZmiLoraPlan w) {
+  constexpr int WK = LORA_WAVES / (WR * WN), RW = RT / WR, NW = NT / WN;
+  constexpr int BLOCKS = KS / 64;                       // 64-element blocks of a stage
+  constexpr int UNITS = (RT + NT) * 2 * BLOCKS;         // 1 KiB each, [block][8 rows]
+  constexpr int OPS = (UNITS + LORA_WAVES - 1) / LORA_WAVES;
+  constexpr int STAGE = UNITS * 1024;
+  static_assert(BLOCKS % WK == 0 && (D - 2) * OPS < 64, "blocks split over wavefronts; the wait counter");
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = lane / 16, c16 = lane % 16;
   Tile t;
-  if (!(SMALL ? lora_find_tile(p, blockIdx.x, t) : lora_planned_tile(w, blockIdx.x, t))) return;
+  if (!(SMALL ? lora_find_tile(p, blockIdx.x, t) : lora_planned_tile(w.tiles, w.header[0], blockIdx.x, t))) return;
   if (t.slot == p.n_slots) return;
   const int rank = lora_rank(p, t.slot), lt = (rank + 15) / 16, live = lt * p.n_slices;
   const int q0 = blockIdx.y * NT;
   if (q0 >= live) return;
-  const uint16_t *xr[RT], *ar[NT];
+  // this lane's pieces of a stage
+  const uint16_t *from[OPS];
+  uint32_t into[OPS];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int at = i * 16 + c16 < t.n ? i * 16 + c16 : 0;
-    const int row = SMALL ? __shfl(t.row, at, 64) : w.order[t.first + at];
-    xr[i] = (const uint16_t *)p.x + row * p.ldx + g * 16;
+  for (int i = 0; i < OPS; ++i) {
+    int u = wave + i * LORA_WAVES;
+    if (u >= UNITS) u = UNITS - 1;                      // (the last unit again: the same bytes to the same place)
+    const int block = u / ((RT + NT) * 2), r = u % ((RT + NT) * 2) * 8 + lane / 8, piece = lane % 8 ^ (lane / 8);
+    into[i] = u * 1024;
+    if (r < RT * 16) {
+      const int at = r < t.n ? r : 0;
+      const int row = SMALL ? __shfl(t.row, at, 64) : w.order[t.first + at];
+      from[i] = (const uint16_t *)p.x + row * p.ldx;
+    } else {
+      const int q = q0 + (r - RT * 16) / 16 < live ? q0 + (r - RT * 16) / 16 : live - 1, s = q / lt;
+      const int k = (q - s * lt) * 16 + r % 16;
+      from[i] = (const uint16_t *)p.a + t.slot * p.a_slot + (s * p.rank + (k < rank ? k : rank - 1)) * p.a_ld;
+    }
+    from[i] += block * 64 + piece * 8;
   }
+  const int stages = (p.K + KS - 1) / KS, full = p.K / KS;
+  const int s0 = (int)((int64_t)stages * blockIdx.z / gridDim.z), s1 = (int)((int64_t)stages * (blockIdx.z + 1) / gridDim.z);
+  f32x4 acc[RW][NW];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int q = q0 + i < live ? q0 + i : live - 1, s = q / lt;
-    const int r = (q - s * lt) * 16 + c16;
-    ar[i] = (const uint16_t *)p.a + t.slot * p.a_slot + (s * p.rank + (r < rank ? r : rank - 1)) * p.a_ld + g * 16;
-  }
-  // K in groups of DEPTH steps of 32 elements: lane group g takes elements g * 16 + 0 .. 7 of a 64-element chunk in its
-  // first step and + 8 .. 15 in its second, so that two steps read whole 128-byte lines
-  constexpr int GROUP = 32 * DEPTH;
-  const int groups = (p.K + GROUP - 1) / GROUP;
-  const int parts = gridDim.z * LORA_WAVES, part = blockIdx.z * LORA_WAVES + wave;
-  const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
-  const int whole = g1 * GROUP <= p.K ? g1 : g1 - 1;
-  f32x4 acc[RT][NT];
+  for (int i = 0; i < RW; ++i)
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int j = 0; j < NW; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  const int wr = wave % WR, wn = wave / WR % WN, wk = wave / (WR * WN);
+  // where this lane's operands stand in a stage: row c16 of 16, slot of piece h * 4 + g
+  const uint32_t at0 = wk * ((RT + NT) * 2048) + c16 / 8 * 1024 + c16 % 8 * 128 + ((uint32_t)g ^ (c16 & 3)) * 16;
+  const uint32_t side = (c16 & 4) * 16;                 // (the slot's upper bit: h ^ bit 2 of the row)
+  auto compute = [&](const char *stage) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  u32x4 xf[DEPTH][RT], af[DEPTH][NT];
-  auto load = [&](u32x4 (&x)[RT], u32x4 (&a)[NT], int64_t k) {
+    for (int b = 0; b < BLOCKS / WK; ++b)
 #pragma unroll
-    for (int j = 0; j < RT; ++j) x[j] = load16(xr[j] + k);
+      for (int h = 0; h < 2; ++h) {
+        const char *at = stage + b * WK * ((RT + NT) * 2048) + at0 + ((h * 64) ^ side);
+        u32x4 x[RW], a[NW];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) a[j] = load16(ar[j] + k);
+        for (int i = 0; i < RW; ++i) x[i] = *(const u32x4 *)(at + (wr * RW + i) * 2048);
+#pragma unroll
+        for (int j = 0; j < NW; ++j) a[j] = *(const u32x4 *)(at + (RT + wn * NW + j) * 2048);
+#pragma unroll
+        for (int j = 0; j < NW; ++j)
+#pragma unroll
+          for (int i = 0; i < RW; ++i) acc[i][j] = mma_x<F16>(a[j], x[i], acc[i][j]);
+      }
   };
-  auto mma = [&](const u32x4 (&x)[RT], const u32x4 (&a)[NT]) {
+  // stage s through registers (the only way where K ends inside it, or without the alignment)
+  u32x4 reg[OPS];
+  auto fetch = [&](int s) {
+    const int64_t k = (int64_t)s * KS;
+    if (s < full) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < OPS; ++i) reg[i] = load16(from[i] + k);
+    } else {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) acc[i][j] = mma_x<F16>(a[j], x[i], acc[i][j]);
-  };
-  if (g0 < whole) {   // DEPTH steps are in flight
-    int64_t k = (int64_t)g0 * GROUP;
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(xf[d], af[d], k + d / 2 * 64 + d % 2 * 8);
-#pragma unroll 1
-    for (int i = g0 + 1; i < whole; ++i) {
-      k += GROUP;
-#pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {
-        mma(xf[d], af[d]);
-        load(xf[d], af[d], k + d / 2 * 64 + d % 2 * 8);
+      for (int i = 0; i < OPS; ++i) {
+        const int u = wave + i * LORA_WAVES < UNITS ? wave + i * LORA_WAVES : UNITS - 1;
+        const int n = p.K - (int)k - u / ((RT + NT) * 2) * 64 - (lane % 8 ^ (lane / 8)) * 8;
+        reg[i] = n >= 8 ? load16(from[i] + k) : load16_head(from[i] + k, n);
       }
     }
+  };
+  auto put = [&](int slot) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) mma(xf[d], af[d]);
-  }
-  if (whole < g1) {   // the last group when it is not whole
-    const int k0 = whole * GROUP;
+    for (int i = 0; i < OPS; ++i) *(u32x4 *)(lora_smem + slot * STAGE + into[i] + lane * 16) = reg[i];
+  };
+  if (DMA) {
+    const int n = (s1 < full ? s1 : full) - s0;
+    auto issue = [&](int i, int slot) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int k = k0 + d / 2 * 64 + d % 2 * 8;
-#pragma unroll
-      for (int j = 0; j < RT; ++j) xf[d][j] = u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < NT; ++j) af[d][j] = u32x4{0, 0, 0, 0};
-      if (k + g * 16 + 8 <= p.K) load(xf[d], af[d], k);
+      for (int k = 0; k < OPS; ++k) {
+        const uint16_t *src = from[k] + (int64_t)(s0 + i) * KS;
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(slot * STAGE + into[k]), "v"(src) : "memory", "m0");
+      }
+    };
+    for (int i = 0; i < D - 1; ++i)
+      if (i < n) issue(i, i);
+    int slot = 0, next = D - 1;
+    for (int i = 0; i < n; ++i) {
+      if (i + D - 2 < n) wait_loads<(D - 2) * OPS>();
+      else wait_loads<0>();
+      group_barrier();
+      if (i + D - 1 < n) issue(i + D - 1, next);
+      compute(lora_smem + slot * STAGE);
+      slot = slot + 1 == D ? 0 : slot + 1;
+      next = next + 1 == D ? 0 : next + 1;
     }
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) mma(xf[d], af[d]);
-    if (p.K % 8) {   // (the first lane group takes what is left)
-      const int n = g == 0 ? p.K % 8 : 0, k = p.K - p.K % 8;
-#pragma unroll
-      for (int j = 0; j < RT; ++j) xf[0][j] = load16_head(xr[j] + k, n);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) af[0][j] = load16_head(ar[j] + k, n);
-      mma(xf[0], af[0]);
+    if (s1 > full) {
+      fetch(full);
+      group_barrier();
+      put(0);
+      group_barrier();
+      compute(lora_smem);
+    }
+  } else {
+    fetch(s0);
+    for (int s = s0; s < s1; ++s) {
+      put((s - s0) & 1);
+      group_barrier();
+      if (s + 1 < s1) fetch(s + 1);
+      compute(lora_smem + ((s - s0) & 1) * STAGE);
     }
   }
   const int kt = (p.rank + 31) / 32;
@@ -281,7 +370,7 @@ __global__ __launch_bounds__(LORA_WAVES * 64, RT * NT < 32 ? 2 : 1) void zmi_lor
       constexpr int TERMS = decltype(terms)::value;
       __bf16 h[TERMS][4];
       split<TERMS>(f, h);
-      char *to = (char *)w.h + (((((int64_t)blockIdx.x * RT + i) * p.n_slices + s) * kt + r / 32) * TERMS) * 1024 +
+      char *to = (char *)w.h + ((((int64_t)(t.group + i) * p.n_slices + s) * kt + r / 32) * TERMS) * 1024 +
                  (r / 8 % 4 * 16 + c16) * 16 + r % 8 * 2;
 #pragma unroll
       for (int k = 0; k < TERMS; ++k) {
@@ -298,44 +387,61 @@ __global__ __launch_bounds__(LORA_WAVES * 64, RT * NT < 32 ? 2 : 1) void zmi_lor
     const int64_t at = (((int64_t)z * gridDim.x + blockIdx.x) * (p.n_slices * ((p.rank + 15) / 16)) + q) * RT + i;
     return w.partial + (at * 64 + lane) * 4;
   };
+  if (WK > 1) {   // the wavefronts' shares of K meet in LDS; the first of each set goes on
+    f32x4 *red = (f32x4 *)lora_smem + lane;
+    group_barrier();
 #pragma unroll
-  for (int f0 = 0; f0 < FRAGS; f0 += PART) {
-    if (f0) __syncthreads();
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
-    for (int f = 0; f < PART; ++f) red[wave][f][lane] = acc[(f0 + f) % RT][(f0 + f) / RT];
-    __syncthreads();
-    for (int f = wave; f < PART; f += LORA_WAVES) {
-      const int i = (f0 + f) % RT, q = q0 + (f0 + f) / RT;
-      if (q >= live || i * 16 >= t.n) continue;
-      const f32x4 v = red[0][f][lane] + red[1][f][lane] + red[2][f][lane] + red[3][f][lane];
-      if (SMALL) {
-        *(f32x4 *)partial(blockIdx.z, i, q) = v;
-      } else if (gridDim.z == 1) {
-        finish(i, q, v);
-      } else {
-        // (written through to device scope, so that the slice that arrives last can read it: see below)
-        uint64_t *to = (uint64_t *)partial(blockIdx.z, i, q);
-        __hip_atomic_store(to, __builtin_bit_cast(uint64_t, u32x2{__float_as_uint(v[0]), __float_as_uint(v[1])}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(to + 1, __builtin_bit_cast(uint64_t, u32x2{__float_as_uint(v[2]), __float_as_uint(v[3])}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      for (int j = 0; j < NW; ++j) red[(wave * RW * NW + i * NW + j) * 64] = acc[i][j];
+    group_barrier();
+    if (wk == 0) {
+#pragma unroll
+      for (int i = 0; i < RW; ++i)
+#pragma unroll
+        for (int j = 0; j < NW; ++j)
+#pragma unroll
+          for (int k = 1; k < WK; ++k) acc[i][j] += red[((wave + k * WR * WN) * RW * NW + i * NW + j) * 64];
     }
   }
-  if (SMALL || gridDim.z == 1) return;
+  const bool split_k = !SMALL && gridDim.z > 1;
+  if (wk == 0) {
+#pragma unroll
+    for (int i = 0; i < RW; ++i)
+#pragma unroll
+      for (int j = 0; j < NW; ++j) {
+        const int rg = wr * RW + i, q = q0 + wn * NW + j;
+        if (q >= live || rg * 16 >= t.n) continue;
+        const f32x4 v = acc[i][j];
+        if (SMALL) {
+          *(f32x4 *)partial(blockIdx.z, rg, q) = v;
+        } else if (!split_k) {
+          finish(rg, q, v);
+        } else {
+          // (written through to device scope, so that the slice that arrives last can read it: see below)
+          uint64_t *to = (uint64_t *)partial(blockIdx.z, rg, q);
+          __hip_atomic_store(to, __builtin_bit_cast(uint64_t, u32x2{__float_as_uint(v[0]), __float_as_uint(v[1])}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_store(to + 1, __builtin_bit_cast(uint64_t, u32x2{__float_as_uint(v[2]), __float_as_uint(v[3])}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+  }
+  if (!split_k) return;
   // The slice that arrives last at the tile's word adds all slices' sums, in slice order, and leaves the operands.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  wait_loads<0>();   // (stores count as well)
+  group_barrier();
+  int *is_last = (int *)lora_smem;
   if (threadIdx.x == 0)
-    is_last = __hip_atomic_fetch_add(w.arrivals + blockIdx.y * gridDim.x + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.z - 1;
+    *is_last = __hip_atomic_fetch_add(w.arrivals + blockIdx.y * gridDim.x + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.z - 1;
   __syncthreads();
-  if (!is_last) return;
-  for (int f = wave; f < FRAGS; f += LORA_WAVES) {
+  if (!*is_last) return;
+  for (int f = wave; f < RT * NT; f += LORA_WAVES) {
     const int i = f % RT, q = q0 + f / RT;
     if (q >= live || i * 16 >= t.n) continue;
     f32x4 v = {0, 0, 0, 0};
     for (unsigned z = 0; z < gridDim.z; ++z) {
-      const uint64_t *from = (const uint64_t *)partial(z, i, q);
-      const u32x2 a = __builtin_bit_cast(u32x2, __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-      const u32x2 b = __builtin_bit_cast(u32x2, __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+      const uint64_t *src = (const uint64_t *)partial(z, i, q);
+      const u32x2 a = __builtin_bit_cast(u32x2, __hip_atomic_load(src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+      const u32x2 b = __builtin_bit_cast(u32x2, __hip_atomic_load(src + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
       v += f32x4{__uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(b[0]), __uint_as_float(b[1])};
     }
     finish(i, q, v);
@@ -343,86 +449,103 @@ __global__ __launch_bounds__(LORA_WAVES * 64, RT * NT < 32 ? 2 : 1) void zmi_lor
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// expand: workgroup (x: 256 columns of a slice, y: tile), 64 columns a wavefront.  MFMA rows are columns of dst, MFMA
-// columns the tile's rows: of 16-column tile j lane l holds n0 + (j / 2) * 32 + (l / 16) * 8 + j % 2 * 4 .. +3 of row l % 16,
-// so that a lane's columns are two runs of eight and every access to base and dst takes 64 contiguous bytes of a row.
+// expand: workgroup (x: columns of a slice, y: tile), 16 NJ columns a wavefront.  MFMA rows are the tile's rows, MFMA
+// columns columns of dst: of column tile j lane l holds column n0 + l % 16 * NJ + j of rows (l / 16) * 4 .. +3, so that
+// a lane's NJ columns lie together and 16 lanes take 32 NJ contiguous bytes of a row.  B stays in registers for all of the
+// tile's 16-row groups.
 // ---------------------------------------------------------------------------------------------------------------
-template <bool F16, int RT, int TERMS, bool D32, bool SMALL>
-__global__ __launch_bounds__(LORA_WAVES * 64) void zmi_lora_expand_kernel(ZmiLora p, ZmiLoraPlan w, int slices) {
-  constexpr int ES = D32 ? 4 : 2;          // bytes of a dst element
-  constexpr int W = D32 ? 2 : 1;           // 16-byte words of a run of eight
+template <bool F16, int NJ, int KT, int TERMS, bool D32, bool SMALL>
+__global__ __launch_bounds__(LORA_WAVES * 64, KT * NJ * (F16 ? 2 : 1) > 16 ? 2 : 3) void zmi_lora_expand_kernel(ZmiLora p, ZmiLoraPlan w, int slices) {
+  constexpr int ES = D32 ? 4 : 2;            // bytes of a dst element
+  constexpr int BYTES = NJ * ES, WORDS = BYTES / 4;   // a lane's run of a row
+  constexpr int COLS = LORA_WAVES * 16 * NJ;
+  typedef uint32_t run_t __attribute__((ext_vector_type(WORDS)));
   const int lane = threadIdx.x % 64, g = lane / 16, c16 = lane % 16;
   Tile t;
-  if (!(SMALL ? lora_find_tile(p, blockIdx.y, t) : lora_planned_tile(w, blockIdx.y, t))) return;
+  if (!(SMALL ? lora_find_tile(p, blockIdx.y, t) : lora_planned_tile(w.wide, w.header[1], blockIdx.y, t))) return;
   int s = 0, blk = blockIdx.x, col0 = 0;
-  while (blk >= (p.N[s] + LORA_COLS - 1) / LORA_COLS) {
-    blk -= (p.N[s] + LORA_COLS - 1) / LORA_COLS;
+  while (blk >= (p.N[s] + COLS - 1) / COLS) {
+    blk -= (p.N[s] + COLS - 1) / COLS;
     col0 += p.N[s++];
   }
-  const int N = p.N[s], n0 = blk * LORA_COLS + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64;
+  const int N = p.N[s], n0 = blk * COLS + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 16 * NJ;
   if (n0 >= N) return;
   const bool none = t.slot == p.n_slots;
   if (none && p.base == p.dst) return;
-  int64_t row[RT];
-  bool have[RT];
+  const int n = n0 + c16 * NJ, cols = N - n < NJ ? N - n : NJ;   // this lane's columns (none where cols <= 0)
+  int rank = 0, kts = 0;
+  float scale = 0.0f;
+  u32x4 b[KT][NJ][F16 ? 2 : 1];
+  if (!none) {
+    rank = lora_rank(p, t.slot);
+    kts = (rank + 31) / 32;
+    scale = p.scales ? p.scales[t.slot] : 1.0f;
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    have[i] = i * 16 + c16 < t.n;
-    const int at = have[i] ? i * 16 + c16 : 0;
-    row[i] = SMALL ? __shfl(t.row, at, 64) : w.order[t.first + at];
+    for (int c = 0; c < KT; ++c)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int at = n + j < N ? n + j : N - 1, left = rank - c * 32 - g * 8;   // ranks that this lane's eight elements may read
+        const uint16_t *br = (const uint16_t *)p.b[s] + t.slot * p.b_slot[s] + at * p.b_ld[s] + c * 32 + g * 8;
+        u32x4 v = left >= 8 ? load16(br) : load16_head(br, left);
+        if (F16) {
+          float f[8];
+          const f16x8 half = __builtin_bit_cast(f16x8, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = (float)half[e];
+          __bf16 q[2][8];
+          split<2>(f, q);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) b[c][j][F16 ? k : 0] = __builtin_bit_cast(u32x4, bf16x8{q[k][0], q[k][1], q[k][2], q[k][3], q[k][4], q[k][5], q[k][6], q[k][7]});
+        } else {
+          b[c][j][0] = v;
+        }
+      }
   }
-  // ---- base ----
-  u32x4 y[RT][2][W];
+  for (int g0 = 0; g0 < t.n; g0 += 16) {
+    // ---- rows and base ----
+    int64_t row[4];
+    run_t y[4];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const int at = g0 + g * 4 + i;
+      row[i] = at >= t.n || cols <= 0 ? -1 : SMALL ? 0 : w.order[t.first + at];
+      if (SMALL) { const int r = __shfl(t.row, g * 4 + i, 64); if (row[i] >= 0) row[i] = r; }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = n0 + h * 32 + g * 8;
+      for (int k = 0; k < WORDS; ++k) y[i][k] = 0;
+    }
+    if (p.base) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) y[i][h][k] = u32x4{0, 0, 0, 0};
-      if (!p.base || !have[i] || n >= N) continue;
-      const char *at = (const char *)p.base + (row[i] * p.ld_base + col0 + n) * ES;
-      if (n + 8 <= N) {
+      for (int i = 0; i < 4; ++i) {
+        if (row[i] < 0) continue;
+        const char *at = (const char *)p.base + (row[i] * p.ld_base + col0 + n) * ES;
+        if (cols == NJ) {
+          __builtin_memcpy(&y[i], at, BYTES);
+        } else {
 #pragma unroll
-        for (int k = 0; k < W; ++k) y[i][h][k] = load16(at + 16 * k);
-      } else if (D32) {
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (n + e < N) y[i][h][e / 4][e % 4] = ((const uint32_t *)at)[e];
-      } else {
-        y[i][h][0] = load16_head((const uint16_t *)at, N - n);
+          for (int e = 0; e < NJ; ++e) {
+            if (e >= cols) continue;
+            if (D32) y[i][e % WORDS] = ((const uint32_t *)at)[e];
+            else y[i][e / 2] |= (uint32_t)((const uint16_t *)at)[e] << (16 * (e % 2));
+          }
+        }
       }
     }
-  f32x4 acc[RT][4];
+    f32x4 acc[NJ];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  float scale = 0.0f;
-  if (!none) {
-    const int rank = lora_rank(p, t.slot), kts = (rank + 31) / 32, kt = (p.rank + 31) / 32;
-    scale = p.scales ? p.scales[t.slot] : 1.0f;
-    const uint16_t *br[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + (j >> 1) * 32 + c16 / 4 * 8 + (j & 1) * 4 + c16 % 4;
-      br[j] = (const uint16_t *)p.b[s] + t.slot * p.b_slot[s] + (n < N ? n : N - 1) * p.b_ld[s] + g * 8;
-    }
-    for (int c = 0; c < kts; ++c) {
-      const int left = rank - c * 32 - g * 8;   // ranks that this lane's eight elements may read
-      u32x4 b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = left >= 8 ? load16(br[j] + c * 32) : load16_head(br[j] + c * 32, left);
-      u32x4 hf[RT][TERMS];
+    for (int c = 0; c < KT; ++c) {
+      if (c >= kts) break;
+      u32x4 h[TERMS];
       if (SMALL) {
         // the K slices' sums as the shrink launch left them: ranks (r % 16 / 4) * 16 + row, four to a lane
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        const int r = c * 32 + g * 8, lt = (rank + 15) / 16;
-        if (left > 0) {
+        const int r = c * 32 + g * 8, lt = (rank + 15) / 16, left = rank - r;
+        if (left > 0 && c16 < t.n) {
           for (int z = 0; z < slices; ++z) {
             const int64_t at = ((int64_t)z * gridDim.y + blockIdx.y) * (p.n_slices * ((p.rank + 15) / 16)) + s * lt + r / 16;
-            const f32x4 *from = (const f32x4 *)w.partial + at * 64 + r % 16 / 4 * 16 + c16;
-            const f32x4 lo = from[0], hi = from[16];
+            const f32x4 *src = (const f32x4 *)w.partial + at * 64 + r % 16 / 4 * 16 + c16;
+            const f32x4 lo = src[0], hi = src[16];
 #pragma unroll
             for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[4 + e] += hi[e]; }
           }
@@ -430,87 +553,61 @@ __global__ __launch_bounds__(LORA_WAVES * 64) void zmi_lora_expand_kernel(ZmiLor
           for (int e = 0; e < 8; ++e)
             if (e >= left) v[e] = 0.0f;
         }
-        __bf16 h[TERMS][8];
-        split<TERMS>(v, h);
+        __bf16 q[TERMS][8];
+        split<TERMS>(v, q);
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k) hf[0][k] = __builtin_bit_cast(u32x4, bf16x8{h[k][0], h[k][1], h[k][2], h[k][3], h[k][4], h[k][5], h[k][6], h[k][7]});
+        for (int k = 0; k < TERMS; ++k) h[k] = __builtin_bit_cast(u32x4, bf16x8{q[k][0], q[k][1], q[k][2], q[k][3], q[k][4], q[k][5], q[k][6], q[k][7]});
       } else {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int k = 0; k < TERMS; ++k)
-            hf[i][k] = ((const u32x4 *)w.h)[(((((int64_t)blockIdx.y * RT + i) * p.n_slices + s) * kt + c) * TERMS + k) * 64 + lane];
+        for (int k = 0; k < TERMS; ++k)
+          h[k] = ((const u32x4 *)w.h)[((((int64_t)(t.group + g0 / 16) * p.n_slices + s) * ((p.rank + 31) / 32) + c) * TERMS + k) * 64 + lane];
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (F16) {
-          float v[8];
-          const f16x8 half = __builtin_bit_cast(f16x8, b[j]);
+      for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = (float)half[e];
-          __bf16 q[2][8];
-          split<2>(v, q);
-          const u32x4 hi = __builtin_bit_cast(u32x4, bf16x8{q[0][0], q[0][1], q[0][2], q[0][3], q[0][4], q[0][5], q[0][6], q[0][7]});
-          const u32x4 lo = __builtin_bit_cast(u32x4, bf16x8{q[1][0], q[1][1], q[1][2], q[1][3], q[1][4], q[1][5], q[1][6], q[1][7]});
+        for (int k = 0; k < TERMS; ++k) acc[j] = mma_x<false>(h[k], b[c][j][0], acc[j]);
+        // (the product of the last terms is beyond the precision kept)
 #pragma unroll
-          for (int i = 0; i < RT; ++i) {
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) acc[i][j] = mma_x<false>(hi, hf[i][k], acc[i][j]);
-            // (the product of the last terms is beyond the precision kept)
-#pragma unroll
-            for (int k = 0; k + 1 < TERMS; ++k) acc[i][j] = mma_x<false>(lo, hf[i][k], acc[i][j]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) acc[i][j] = mma_x<false>(b[j], hf[i][k], acc[i][j]);
-        }
+        for (int k = 0; F16 && k + 1 < TERMS; ++k) acc[j] = mma_x<false>(h[k], b[c][j][F16 ? 1 : 0], acc[j]);
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = n0 + h * 32 + g * 8;
-      if (!have[i] || n >= N) continue;
-      u32x4 out[W];
+    for (int i = 0; i < 4; ++i) {
+      if (row[i] < 0) continue;
+      run_t out;
       if (none) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) out[k] = y[i][h][k];
+        out = y[i];
       } else if (D32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          out[e / 4][e % 4] = __float_as_uint(__builtin_fmaf(scale, acc[i][2 * h + e / 4][e % 4], __uint_as_float(y[i][h][e / 4][e % 4])));
+        for (int e = 0; e < NJ; ++e) out[e % WORDS] = __float_as_uint(__builtin_fmaf(scale, acc[e][i], __uint_as_float(y[i][e % WORDS])));
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t old = y[i][h][0][e];
-          const float d0 = acc[i][2 * h + e / 2][e % 2 * 2], d1 = acc[i][2 * h + e / 2][e % 2 * 2 + 1];
+        for (int e = 0; e < WORDS; ++e) {
+          const uint32_t old = y[i][e];
+          const float d0 = acc[2 * e % NJ][i], d1 = acc[(2 * e + 1) % NJ][i];
           if (p.dt_dst == ZMI_DT_BF16) {
-            out[0][e] = zmi_pack_bf16(__builtin_fmaf(scale, d0, zmi_bf16_to_f32((uint16_t)old)),
-                                      __builtin_fmaf(scale, d1, zmi_bf16_to_f32((uint16_t)(old >> 16))));
+            out[e] = zmi_pack_bf16(__builtin_fmaf(scale, d0, zmi_bf16_to_f32((uint16_t)old)),
+                                   __builtin_fmaf(scale, d1, zmi_bf16_to_f32((uint16_t)(old >> 16))));
           } else {
-            const _Float16 a = (_Float16)__builtin_fmaf(scale, d0, zmi_f16_to_f32((uint16_t)old));
-            const _Float16 b = (_Float16)__builtin_fmaf(scale, d1, zmi_f16_to_f32((uint16_t)(old >> 16)));
-            out[0][e] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+            const _Float16 lo = (_Float16)__builtin_fmaf(scale, d0, zmi_f16_to_f32((uint16_t)old));
+            const _Float16 hi = (_Float16)__builtin_fmaf(scale, d1, zmi_f16_to_f32((uint16_t)(old >> 16)));
+            out[e] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | (uint32_t)__builtin_bit_cast(uint16_t, hi) << 16;
           }
         }
       }
       char *at = (char *)p.dst + (row[i] * p.ld_dst + col0 + n) * ES;
-      if (n + 8 <= N) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) store16(at + 16 * k, out[k]);
+      if (cols == NJ) {
+        __builtin_memcpy(at, &out, BYTES);
       } else {
 #pragma unroll
-        for (int e = 0; e < 7; ++e) {
-          if (n + e >= N) continue;
-          if (D32) ((uint32_t *)at)[e] = out[e / 4][e % 4];
-          else ((uint16_t *)at)[e] = (uint16_t)(out[0][e / 2] >> (16 * (e % 2)));
+        for (int e = 0; e < NJ; ++e) {
+          if (e >= cols) continue;
+          if (D32) ((uint32_t *)at)[e] = out[e % WORDS];
+          else ((uint16_t *)at)[e] = (uint16_t)(out[e / 2] >> (16 * (e % 2)));
         }
       }
     }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -518,13 +615,22 @@ namespace {
 
 struct Shape {
   bool small;
+  bool dma;          // rows of x and A and their addresses are 16-byte multiples
   int rt;            // 16-row groups of a tile
   int nt;            // rank tiles of a shrink workgroup
   int ny;            // shrink workgroups over the rank tiles
   int ks;            // K slices
   int64_t tiles;     // tiles there can be
+  int kt;            // 32-rank blocks an expand wavefront holds
+  int nj;            // its column tiles
+  int wide;          // tiles of an expand workgroup
+  int64_t wide_tiles;
+  int64_t col_blocks;
   int terms;
 };
+
+// elements of K in a stage of the shrink launch: a stage is 10 .. 24 KiB whatever the tile's shape
+constexpr int lora_ks(int rt, int nt) { return rt + nt <= 3 ? (rt + nt == 2 ? 256 : rt == 1 ? 256 : 128) : rt == 1 && nt == 4 ? 128 : rt == 2 && nt == 2 ? 128 : 64; }
 
 Shape lora_shape(const ZmiLora &p) {
   Shape s;
@@ -536,11 +642,20 @@ Shape lora_shape(const ZmiLora &p) {
   const int qt = p.n_slices * ((p.rank + 15) / 16);
   s.nt = qt >= 8 ? 8 : qt > 2 ? 4 : qt;
   s.ny = (qt + s.nt - 1) / s.nt;
-  int64_t want = 512 / (s.tiles * s.ny), most = (p.K + 255) / 256 / LORA_WAVES;
+  const int stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
+  int64_t want = 512 / (s.tiles * s.ny), most = stages / 4;
   s.ks = (int)(want < most ? want : most);
   if (s.ks > 16) s.ks = 16;
   if (s.ks < 1) s.ks = 1;
   s.terms = p.dt_dst == ZMI_DT_F32 ? 3 : 2;
+  s.dma = p.ldx % 8 == 0 && p.a_ld % 8 == 0 && p.a_slot % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
+  s.kt = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : p.rank <= 128 ? 4 : 8;
+  s.nj = s.small || s.terms == 3 || s.kt == 8 || p.dt_x == ZMI_DT_F16 ? (s.kt == 8 && p.dt_x == ZMI_DT_F16 ? 2 : 4) : 8;
+  s.col_blocks = 0;
+  const int cols = LORA_WAVES * 16 * s.nj;
+  for (int i = 0; i < p.n_slices; ++i) s.col_blocks += (p.N[i] + cols - 1) / cols;
+  s.wide = s.col_blocks * s.tiles >= 4 * 512 ? 4 : s.col_blocks * s.tiles >= 2 * 512 ? 2 : 1;
+  s.wide_tiles = ids + (p.T - ids) / (16 * s.rt * s.wide);
   return s;
 }
 
@@ -555,7 +670,9 @@ size_t lora_layout(const ZmiLora &p, const Shape &s, char *base, ZmiLoraPlan *w)
   if (!s.small) {
     l.header = (int32_t *)take(16);
     l.tiles = (int32_t *)take((size_t)s.tiles * 16);
+    l.wide = (int32_t *)take((size_t)s.wide_tiles * 16);
     l.order = (int32_t *)take((size_t)p.T * 4);
+    l.place = (int32_t *)take(p.T > LORA_PLAN_KEEP * 1024 ? (size_t)p.T * 4 : 0);
     l.n_arrivals = (int32_t)(s.tiles * s.ny);
     l.arrivals = (uint32_t *)take((size_t)l.n_arrivals * 4);
     l.h = take((size_t)s.tiles * s.rt * p.n_slices * ((p.rank + 31) / 32) * s.terms * 1024);
@@ -565,40 +682,58 @@ size_t lora_layout(const ZmiLora &p, const Shape &s, char *base, ZmiLoraPlan *w)
   return at;
 }
 
-template <bool F16, int RT, bool SMALL>
-void launch_shrink(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+template <bool F16, int RT, int NT, int WR, int WN, bool SMALL>
+hipError_t launch_shrink_as(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+  constexpr int KS = lora_ks(RT, NT), STAGE = (RT + NT) * 32 * KS, D = STAGE <= 18432 ? 4 : 3;
+  static_assert(LORA_WAVES / (WR * WN) * WR * WN == LORA_WAVES && D * STAGE <= 80 * 1024, "two workgroups a compute unit");
   const dim3 grid((unsigned)s.tiles, (unsigned)s.ny, (unsigned)s.ks), block(LORA_WAVES * 64);
-  constexpr int D1 = RT == 4 ? 4 : 8, D4 = RT == 4 ? 2 : 4;
-  if (s.nt == 1) hipLaunchKernelGGL((zmi_lora_shrink_kernel<F16, RT, 1, D1, SMALL>), grid, block, 0, stream, p, w);
-  else if (s.nt == 2) hipLaunchKernelGGL((zmi_lora_shrink_kernel<F16, RT, 2, 4, SMALL>), grid, block, 0, stream, p, w);
-  else if (s.nt == 4) hipLaunchKernelGGL((zmi_lora_shrink_kernel<F16, RT, 4, D4, SMALL>), grid, block, 0, stream, p, w);
-  else hipLaunchKernelGGL((zmi_lora_shrink_kernel<F16, RT, 8, 2, SMALL>), grid, block, 0, stream, p, w);
+  if (s.dma) {
+    const auto kernel = zmi_lora_shrink_kernel<F16, RT, NT, KS, WR, WN, D, true, SMALL>;
+    const hipError_t e = zmi_func_smem_once((const void *)kernel, D * STAGE);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, grid, block, D * STAGE, stream, p, w);
+  } else {
+    const auto kernel = zmi_lora_shrink_kernel<F16, RT, NT, KS, WR, WN, D, false, SMALL>;
+    hipLaunchKernelGGL(kernel, grid, block, 2 * STAGE, stream, p, w);
+  }
+  return hipGetLastError();
 }
 
 template <bool F16, int RT, bool SMALL>
-void launch_expand(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
-  int64_t blocks = 0;
-  for (int i = 0; i < p.n_slices; ++i) blocks += (p.N[i] + LORA_COLS - 1) / LORA_COLS;
-  const dim3 grid((unsigned)blocks, (unsigned)s.tiles), block(LORA_WAVES * 64);
-  if (p.dt_dst == ZMI_DT_F32) hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, RT, 3, true, SMALL>), grid, block, 0, stream, p, w, s.ks);
-  else hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, RT, 2, false, SMALL>), grid, block, 0, stream, p, w, s.ks);
+hipError_t launch_shrink(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+  constexpr int R2 = RT >= 2 ? 2 : 1;
+  if (s.nt == 1) return launch_shrink_as<F16, RT, 1, RT, 1, SMALL>(p, w, s, stream);
+  if (s.nt == 2) return launch_shrink_as<F16, RT, 2, RT, RT == 2 ? 2 : 1, SMALL>(p, w, s, stream);
+  if (s.nt == 4) return launch_shrink_as<F16, RT, 4, R2, 4 / R2, SMALL>(p, w, s, stream);
+  return launch_shrink_as<F16, RT, 8, R2, 4 / R2, SMALL>(p, w, s, stream);
+}
+
+template <bool F16, bool SMALL, int NJ, int KT, bool D32>
+hipError_t launch_expand_as(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+  const dim3 grid((unsigned)s.col_blocks, (unsigned)(SMALL ? s.tiles : s.wide_tiles)), block(LORA_WAVES * 64);
+  hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, NJ, KT, D32 ? 3 : 2, D32, SMALL>), grid, block, 0, stream, p, w, s.ks);
+  return hipGetLastError();
+}
+
+template <bool F16, bool SMALL, int KT>
+hipError_t launch_expand_kt(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+  constexpr int FEW = KT == 8 && F16 ? 2 : 4, NJ = SMALL || F16 || KT == 8 ? FEW : 8;
+  if (s.terms == 3) return launch_expand_as<F16, SMALL, FEW, KT, true>(p, w, s, stream);
+  return launch_expand_as<F16, SMALL, NJ, KT, false>(p, w, s, stream);
+}
+
+template <bool F16, bool SMALL>
+hipError_t launch_expand(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+  return s.kt == 1 ? launch_expand_kt<F16, SMALL, 1>(p, w, s, stream) : s.kt == 2 ? launch_expand_kt<F16, SMALL, 2>(p, w, s, stream)
+       : s.kt == 4 ? launch_expand_kt<F16, SMALL, 4>(p, w, s, stream) : launch_expand_kt<F16, SMALL, 8>(p, w, s, stream);
 }
 
 template <bool F16>
-void launch_both(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
-  if (s.small) {
-    launch_shrink<F16, 1, true>(p, w, s, stream);
-    launch_expand<F16, 1, true>(p, w, s, stream);
-  } else if (s.rt == 1) {
-    launch_shrink<F16, 1, false>(p, w, s, stream);
-    launch_expand<F16, 1, false>(p, w, s, stream);
-  } else if (s.rt == 2) {
-    launch_shrink<F16, 2, false>(p, w, s, stream);
-    launch_expand<F16, 2, false>(p, w, s, stream);
-  } else {
-    launch_shrink<F16, 4, false>(p, w, s, stream);
-    launch_expand<F16, 4, false>(p, w, s, stream);
-  }
+hipError_t launch_both(const ZmiLora &p, const ZmiLoraPlan &w, const Shape &s, hipStream_t stream) {
+  const hipError_t e = s.small ? launch_shrink<F16, 1, true>(p, w, s, stream) : s.rt == 1 ? launch_shrink<F16, 1, false>(p, w, s, stream)
+                     : s.rt == 2 ? launch_shrink<F16, 2, false>(p, w, s, stream) : launch_shrink<F16, 4, false>(p, w, s, stream);
+  if (e != hipSuccess) return e;
+  return s.small ? launch_expand<F16, true>(p, w, s, stream) : launch_expand<F16, false>(p, w, s, stream);
 }
 
 }  // namespace
@@ -612,9 +747,7 @@ hipError_t zmi_launch_lora(const ZmiLora &p, hipStream_t stream, const char **na
   if (s.tiles > 65535 || s.ny > 65535) return hipErrorInvalidValue;
   ZmiLoraPlan w;
   lora_layout(p, s, (char *)p.workspace, &w);
-  if (!s.small) hipLaunchKernelGGL(zmi_lora_plan_kernel, dim3(1), dim3(1024), 0, stream, p, w, 16 * s.rt);
-  if (p.dt_x == ZMI_DT_F16) launch_both<true>(p, w, s, stream);
-  else launch_both<false>(p, w, s, stream);
+  if (!s.small) hipLaunchKernelGGL(zmi_lora_plan_kernel, dim3(1), dim3(1024), 0, stream, p, w, 16 * s.rt, s.wide);
   *name = s.small ? "lora_small" : "lora_planned";
-  return hipGetLastError();
+  return p.dt_x == ZMI_DT_F16 ? launch_both<true>(p, w, s, stream) : launch_both<false>(p, w, s, stream);
 }

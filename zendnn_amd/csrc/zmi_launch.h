@@ -348,9 +348,11 @@ struct ZmiLora {
 #define ZMI_LORA_MAX_SLOTS 4096
 // the parts of the workspace
 struct ZmiLoraPlan {
-  int32_t *header;            // number of tiles
-  int32_t *tiles;             // {slot, first position in `order`, rows, unused} of each
+  int32_t *header;            // number of tiles, of wide tiles
+  int32_t *tiles;             // {slot, first position in `order`, rows, number of the first 16-row group} of each
+  int32_t *wide;              // the same of the expand launch's tiles
   int32_t *order;             // [T] rows sorted by slot
+  int32_t *place;             // (the plan launch's own)
   uint32_t *arrivals;         // a word per tile and group of rank tiles, zeroed by the plan launch
   void *h;                    // h as MFMA operands
   float *partial;             // the K slices' sums
