@@ -74,7 +74,7 @@ def test_router_refusals(kw, status, text):
     (dict(N=(32, 0)), capi.FAILURE, "bad sizes"), (dict(N=(8,) * 5), capi.UNIMPLEMENTED, "4 slices"),
     (dict(rank=257), capi.UNIMPLEMENTED, "256"), (dict(n_slots=4097), capi.UNIMPLEMENTED, "slots"),
     (dict(N=(0x7fffffff, 0x7fffffff)), capi.UNIMPLEMENTED, "columns"),
-    (dict(T=(1 << 20) + 1), capi.UNIMPLEMENTED, "rows"),
+    (dict(T=(1 << 20) + 1), capi.UNIMPLEMENTED, "rows"), (dict(K=(1 << 19) + 1), capi.UNIMPLEMENTED, "2^19"),
     (dict(dt_x=capi.DT_F32), capi.UNIMPLEMENTED, "dt_x"), (dict(dt_dst=capi.DT_S8), capi.UNIMPLEMENTED, "dt_dst"),
     (dict(x=None), capi.FAILURE, "null"), (dict(slot_ids=None), capi.FAILURE, "null"), (dict(dst=None), capi.FAILURE, "null"),
     (dict(a=None), capi.FAILURE, "a is null"), (dict(a_ld=63), capi.FAILURE, "a is null"),

@@ -19,7 +19,8 @@ int32_t lora_check_sizes(const zmi_lora_t &l) {
     cols += l.N[s];
   }
   if (cols > 0x7fffff00) { set_error("lora: too many columns"); return ZMI_UNIMPLEMENTED; }
-  if (l.T > 1 << 20) { set_error("lora: at most 2^20 rows"); return ZMI_UNIMPLEMENTED; }
+  // (tiles x rank tile sets x stages of K stay below 2^31: 20.5 k x 8 x 8192)
+  if (l.T > 1 << 20 || l.K > 1 << 19) { set_error("lora: at most 2^20 rows, K at most 2^19"); return ZMI_UNIMPLEMENTED; }
   if (!half_type(l.dt_x)) { set_error("lora: dt_x must be bf16 or f16"); return ZMI_UNIMPLEMENTED; }
   if (!half_type(l.dt_dst) && l.dt_dst != ZMI_DT_F32) { set_error("lora: dt_dst must be bf16, f16 or f32"); return ZMI_UNIMPLEMENTED; }
   return ZMI_SUCCESS;

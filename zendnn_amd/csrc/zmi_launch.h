@@ -348,14 +348,14 @@ struct ZmiLora {
 #define ZMI_LORA_MAX_SLOTS 4096
 // the parts of the workspace
 struct ZmiLoraPlan {
-  int32_t *header;            // number of tiles, of wide tiles
-  int32_t *tiles;             // {slot, first position in `order`, rows, number of the first 16-row group} of each
-  int32_t *wide;              // the same of the expand launch's tiles
-  int32_t *order;             // [T] rows sorted by slot
+  int32_t *header;            // number of tiles, of 16-row groups with an adapter, of all groups
+  int32_t *tiles;             // {slot, number of its first group, rows, rank} of each shrink tile
+  int32_t *group_slot;        // {slot, rank} of each group
+  int32_t *order;             // the groups' rows, 16 each, -1: none
   int32_t *place;             // (the plan launch's own)
-  uint32_t *arrivals;         // a word per tile and group of rank tiles, zeroed by the plan launch
+  uint32_t *arrivals;         // a word per tile and set of rank tiles, zeroed by the plan launch
   void *h;                    // h as MFMA operands
-  float *partial;             // the K slices' sums
+  float *partial;             // sums over parts of K
   int32_t n_arrivals;
 };
 size_t zmi_lora_workspace_bytes(const ZmiLora &p);   // (goes by the sizes and types only)
