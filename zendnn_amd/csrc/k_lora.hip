@@ -39,17 +39,18 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
   int *count = (int *)lora_smem;   // [waves][n]
   const int share = (p.T + waves * 64 - 1) / (waves * 64) * 64;   // rows of a wavefront
   const int t0 = wave < waves ? wave * share : p.T, t1 = t0 + share < p.T ? t0 + share : p.T;
-  auto slot_of = [&](int t) {
-    if (t >= t1) return -1;
-    const int id = p.slot_ids[t];
-    return (unsigned)id < (unsigned)p.n_slots ? id : p.n_slots;
-  };
+  auto slot_of = [&](int t, int raw) { return t >= t1 ? -1 : (unsigned)raw < (unsigned)p.n_slots ? raw : p.n_slots; };
   int id[LORA_PLAN_KEEP], pos[LORA_PLAN_KEEP];
 #pragma unroll
-  for (int i = 0; i < LORA_PLAN_KEEP; ++i) id[i] = slot_of(t0 + i * 64 + lane);
+  for (int i = 0; i < LORA_PLAN_KEEP; ++i) {   // (all loads in flight: no branch in front of them)
+    const int t = t0 + i * 64 + lane;
+    id[i] = p.slot_ids[t < p.T ? t : p.T - 1];
+  }
   for (int i = tid; i < waves * n; i += 1024) count[i] = 0;
   for (int i = tid; i < w.n_arrivals; i += 1024) w.arrivals[i] = 0;
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < LORA_PLAN_KEEP; ++i) id[i] = slot_of(t0 + i * 64 + lane, id[i]);
   const int bits = 32 - __builtin_clz(n);
   int *mine = count + (wave < waves ? wave : 0) * n;
   auto place = [&](int slot) {
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
   for (int i = 0; i < LORA_PLAN_KEEP; ++i)
     if (t0 + i * 64 < t1) pos[i] = place(id[i]);
   for (int t = t0 + LORA_PLAN_KEEP * 64; t < t1; t += 64) {
-    const int at = place(slot_of(t + lane));
+    const int at = place(slot_of(t + lane, p.slot_ids[t + lane < p.T ? t + lane : p.T - 1]));
     if (t + lane < t1) w.place[t + lane] = at;
   }
   __syncthreads();
@@ -84,11 +85,13 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
     const int i = tid * per + k;
     total[k] = 0;
     if (k >= per || i >= n) continue;
-    int c = 0;   // its rows; a wavefront's count becomes the number of rows before its own
-    for (int v = 0; v < waves; ++v) {
-      const int own = count[v * n + i];
-      count[v * n + i] = c;
-      c += own;
+    int c = 0, own[16];   // its rows; a wavefront's count becomes the number of rows before its own
+#pragma unroll
+    for (int v = 0; v < 16; ++v) own[v] = v < waves ? count[v * n + i] : 0;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      if (v < waves) count[v * n + i] = c;
+      c += own[v];
     }
     total[k] = c;
     sums[0] += (c + 15) / 16;
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
   }
   __syncthreads();
   // (each lane reads back the places that it wrote itself)
-  for (int t = t0 + LORA_PLAN_KEEP * 64 + lane; t < t1; t += 64) w.order[mine[slot_of(t)] + w.place[t]] = t;
+  for (int t = t0 + LORA_PLAN_KEEP * 64 + lane; t < t1; t += 64) w.order[mine[slot_of(t, p.slot_ids[t])] + w.place[t]] = t;
 #pragma unroll
   for (int i = 0; i < LORA_PLAN_KEEP; ++i)
     if (id[i] >= 0) w.order[mine[id[i]] + pos[i]] = t0 + i * 64 + lane;
@@ -374,17 +377,33 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
         *is_last = __hip_atomic_fetch_add(w.arrivals + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(hi - lo);
       __syncthreads();
       if (*is_last) {
-        for (int f = wave; f < RT * NT; f += LORA_WAVES) {
-          const int i = f % RT, j = f / RT;
-          if (q0 + j >= live || i * 16 >= t.n) continue;
-          f32x4 v = {0, 0, 0, 0};
-          for (int who = lo; who <= hi; ++who) {
-            const uint64_t *src = (const uint64_t *)piece_at(who, i, j);
-            const u32x2 a = __builtin_bit_cast(u32x2, __hip_atomic_load(src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-            const u32x2 b = __builtin_bit_cast(u32x2, __hip_atomic_load(src + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-            v += f32x4{__uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(b[0]), __uint_as_float(b[1])};
-          }
-          finish(i, q0 + j, v);
+        // (a wavefront's fragments of two pieces are asked for together: the loads are what this takes)
+        constexpr int MINE = (RT * NT + LORA_WAVES - 1) / LORA_WAVES;
+        f32x4 v[MINE];
+#pragma unroll
+        for (int f = 0; f < MINE; ++f) v[f] = f32x4{0, 0, 0, 0};
+        for (int who = lo; who <= hi; who += 2) {
+          u32x4 got[2][MINE];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int f = 0; f < MINE; ++f) {
+              const int at = wave + f * LORA_WAVES < RT * NT ? wave + f * LORA_WAVES : RT * NT - 1;
+              const uint64_t *src = (const uint64_t *)piece_at(who + k <= hi ? who + k : hi, at % RT, at / RT);
+              const u32x2 a = __builtin_bit_cast(u32x2, __hip_atomic_load(src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+              const u32x2 b = __builtin_bit_cast(u32x2, __hip_atomic_load(src + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+              got[k][f] = u32x4{a[0], a[1], b[0], b[1]};
+            }
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int f = 0; f < MINE; ++f)
+              if (who + k <= hi) v[f] += __builtin_bit_cast(f32x4, got[k][f]);
+        }
+#pragma unroll
+        for (int f = 0; f < MINE; ++f) {
+          const int at = wave + f * LORA_WAVES, i = at % RT, q = q0 + at / RT;
+          if (at < RT * NT && q < live && i * 16 < t.n) finish(i, q, v[f]);
         }
       }
     }
@@ -414,8 +433,9 @@ LoraShape lora_shape(const ZmiLora &p) {
   const int64_t stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
   // small: K slices of four stages or more while there is less than two workgroups a compute unit
   s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages / 4, 1, 16));
-  // planned: two workgroups a compute unit, runs of four stages or more
-  s.grid = (int)lora_clamp(s.tiles * s.ny * stages / 4, 8, 512) / 8 * 8;
+  // planned: a workgroup a compute unit (two share what one already gets through: 512 workgroups 90 us against 82 for 8192
+  // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of eight stages or more
+  s.grid = (int)lora_clamp(s.tiles * s.ny * stages / 8, 8, 256) / 8 * 8;
   s.terms = p.dt_dst == ZMI_DT_F32 ? 3 : 2;
   s.dma = p.ldx % 8 == 0 && p.a_ld % 8 == 0 && p.a_slot % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
   s.kt = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : p.rank <= 128 ? 4 : 8;
