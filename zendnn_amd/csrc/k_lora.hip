@@ -6,7 +6,7 @@
 // multiply-adds, so HBM bounds every size, and latency the small ones.  Rows of one slot are gathered into tiles of
 // 16 RT rows, so that a tile reads its slot's A and B once and both products run on the 16 x 16 x 32 MFMA:
 //
-//   plan    (more than 64 rows) one workgroup sorts the rows by slot and lists the tiles; up to 64 rows every
+//   plan    (many rows) one workgroup sorts the rows by slot and lists the tiles; with few rows every
 //           wavefront finds its tile by itself from a ballot per distinct id, and there is no such launch;
 //   shrink  h of a tile, K through an LDS ring.  K is cut into slices where the tiles alone do not fill the device;
 //   expand  dst.  A wavefront keeps 32 .. 128 columns' B in registers and goes down the rows of its slot.
@@ -17,6 +17,8 @@
 #include <type_traits>
 
 #include "zmi_lora.h"
+
+#define LORA_RUN 4   // least stages of a shrink workgroup's run
 
 namespace {
 
@@ -36,7 +38,8 @@ extern __shared__ __attribute__((aligned(16))) char lora_smem[];
 __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraPlan w, int tile, int waves) {
   __shared__ int wave_sums[2][16];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = p.n_slots + 1;
-  int *count = (int *)lora_smem;   // [waves][n]
+  int4 *of = (int4 *)lora_smem;                // [n]
+  int *count = (int *)(lora_smem + n * 16);   // [waves][n]
   const int share = (p.T + waves * 64 - 1) / (waves * 64) * 64;   // rows of a wavefront
   const int t0 = wave < waves ? wave * share : p.T, t1 = t0 + share < p.T ? t0 + share : p.T;
   auto slot_of = [&](int t, int raw) { return t >= t1 ? -1 : (unsigned)raw < (unsigned)p.n_slots ? raw : p.n_slots; };
@@ -49,6 +52,13 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
   for (int i = tid; i < waves * n; i += 1024) count[i] = 0;
   for (int i = tid; i < w.n_arrivals; i += 1024) w.arrivals[i] = 0;
   __syncthreads();
+  constexpr int MOST = (ZMI_LORA_MAX_SLOTS + 1 + 1023) / 1024;   // slots of a thread
+  int total[MOST], rank[MOST];
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    const int i = tid * ((n + 1023) / 1024) + k;
+    rank[k] = k < (n + 1023) / 1024 && i < p.n_slots ? lora_rank(p, i) : 0;
+  }
 #pragma unroll
   for (int i = 0; i < LORA_PLAN_KEEP; ++i) id[i] = slot_of(t0 + i * 64 + lane, id[i]);
   const int bits = 32 - __builtin_clz(n);
@@ -78,8 +88,6 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
   // thread i owns slots [i per, (i + 1) per)
   const int per = (n + 1023) / 1024;
   int sums[2] = {0, 0};   // 16-row groups, tiles
-  constexpr int MOST = (ZMI_LORA_MAX_SLOTS + 1 + 1023) / 1024;
-  int total[MOST];
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     const int i = tid * per + k;
@@ -110,33 +118,39 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
     start[k] = v - sums[k];
   }
   __syncthreads();
-  for (int i = 0; i < wave; ++i)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) start[k] += wave_sums[k][i];
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) start[k] += i < wave ? wave_sums[k][i] : 0;
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     const int i = tid * per + k;
     if (k >= per || i >= n) continue;
-    const int c = total[k], groups = (c + 15) / 16, rank = i < p.n_slots && c ? lora_rank(p, i) : 0;
+    of[i] = make_int4(start[0], start[1], total[k], rank[k]);
+    start[0] += (total[k] + 15) / 16;
     if (i == p.n_slots) {   // (the rows without an adapter)
       w.header[0] = start[1];
-      w.header[1] = start[0];
-      w.header[2] = start[0] + groups;
-    } else {
-      for (int j = 0; j < c; j += tile)
-        *(int4 *)(w.tiles + 4 * (int64_t)start[1]++) = make_int4(i, start[0] + j / 16, c - j < tile ? c - j : tile, rank);
+      w.header[1] = start[0] - (total[k] + 15) / 16;
+      w.header[2] = start[0];
     }
-    for (int j = 0; j < groups; ++j) *(int2 *)(w.group_slot + 2 * (int64_t)(start[0] + j)) = make_int2(i, rank);
-    for (int j = c; j < groups * 16; ++j) w.order[(int64_t)start[0] * 16 + j] = -1;
-    for (int v = 0; v < waves; ++v) count[v * n + i] += start[0] * 16;
-    start[0] += groups;
+    start[1] += (total[k] + tile - 1) / tile;
   }
   __syncthreads();
+  // every row to its place; the first of a group or tile writes its entry, a slot's last row the empty places behind it
+  auto put = [&](int t, int slot, int at) {
+    const int4 o = of[slot];   // first group, first tile, rows, rank
+    const int q = mine[slot] + at;
+    w.order[(int64_t)o.x * 16 + q] = t;
+    if (q % 16 == 0) *(int2 *)(w.group_slot + 2 * (int64_t)(o.x + q / 16)) = make_int2(slot, o.w);
+    if (q % tile == 0 && slot < p.n_slots) *(int4 *)(w.tiles + 4 * (int64_t)(o.y + q / tile)) = make_int4(slot, o.x + q / 16, o.z - q < tile ? o.z - q : tile, o.w);
+    if (q == o.z - 1)
+      for (int j = q + 1; j % 16; ++j) w.order[(int64_t)o.x * 16 + j] = -1;
+  };
   // (each lane reads back the places that it wrote itself)
-  for (int t = t0 + LORA_PLAN_KEEP * 64 + lane; t < t1; t += 64) w.order[mine[slot_of(t, p.slot_ids[t])] + w.place[t]] = t;
+  for (int t = t0 + LORA_PLAN_KEEP * 64 + lane; t < t1; t += 64) put(t, slot_of(t, p.slot_ids[t]), w.place[t]);
 #pragma unroll
   for (int i = 0; i < LORA_PLAN_KEEP; ++i)
-    if (id[i] >= 0) w.order[mine[id[i]] + pos[i]] = t0 + i * 64 + lane;
+    if (id[i] >= 0) put(t0 + i * 64 + lane, id[i], pos[i]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -175,7 +189,13 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
     Tile t;
     int q0, s0, s1;
     if (SMALL) {
-      if (!lora_find_tile(p, blockIdx.x, t) || t.slot == p.n_slots) return;
+      const bool found = lora_find_tile(p, blockIdx.x, t);
+      if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0) {   // the expand launch's entry: {slot, rows, rank, -}, 16 rows
+        int32_t *e = w.tiles + blockIdx.x * 20;
+        if (lane == 0) *(int4 *)e = found ? make_int4(t.slot, t.n, t.slot < p.n_slots ? lora_rank(p, t.slot) : 0, 0) : make_int4(0, 0, 0, 0);
+        if (found && lane < 16) e[4 + lane] = lane < t.n ? t.row : -1;
+      }
+      if (!found || t.slot == p.n_slots) return;
       q0 = blockIdx.y * NT;
       s0 = (int)((int64_t)stages * blockIdx.z / gridDim.z);
       s1 = (int)((int64_t)stages * (blockIdx.z + 1) / gridDim.z);
@@ -242,6 +262,10 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
     };
     // stage s through registers (the only way where K ends inside it, or without the alignment)
     u32x4 reg[OPS];
+    auto left = [&](int i, int k) {   // elements of K from this lane's piece on
+      const int u = wave + i * LORA_WAVES < UNITS ? wave + i * LORA_WAVES : UNITS - 1;
+      return p.K - k - u / ((RT + NT) * 2) * 64 - (lane % 8 ^ (lane / 8)) * 8;
+    };
     auto fetch = [&](int s) {
       const int64_t k = (int64_t)s * KS;
       if (s < full) {
@@ -250,9 +274,13 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
       } else {
 #pragma unroll
         for (int i = 0; i < OPS; ++i) {
-          const int u = wave + i * LORA_WAVES < UNITS ? wave + i * LORA_WAVES : UNITS - 1;
-          const int n = p.K - (int)k - u / ((RT + NT) * 2) * 64 - (lane % 8 ^ (lane / 8)) * 8;
-          reg[i] = n >= 8 ? load16(from[i] + k) : load16_head(from[i] + k, n);
+          reg[i] = u32x4{0, 0, 0, 0};
+          if (left(i, (int)k) >= 8) reg[i] = load16(from[i] + k);
+        }
+        if (p.K % 8) {
+#pragma unroll
+          for (int i = 0; i < OPS; ++i)
+            if (left(i, (int)k) > 0 && left(i, (int)k) < 8) reg[i] = load16_head(from[i] + k, left(i, (int)k));
         }
       }
     };
@@ -415,13 +443,13 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
 namespace {
 
 // elements of K in a stage of the shrink launch: a stage is 10 .. 24 KiB whatever the tile's shape
-constexpr int lora_ks(int rt, int nt) { return rt + nt <= 3 ? (rt + nt == 2 ? 256 : rt == 1 ? 256 : 128) : rt == 1 && nt == 4 ? 128 : rt == 2 && nt == 2 ? 128 : 64; }
+constexpr int lora_ks(int rt, int nt) { return rt + nt <= 3 ? 256 : rt + nt <= 6 ? 128 : 64; }
 
 int64_t lora_clamp(int64_t v, int64_t lo, int64_t hi) { return v > hi ? (hi < lo ? lo : hi) : v < lo ? lo : v; }
 
 LoraShape lora_shape(const ZmiLora &p) {
   LoraShape s = {};
-  s.small = p.T <= LORA_SMALL_T;
+  s.small = p.T <= LORA_SMALL_T || (p.T <= LORA_SMALL_MOST && p.n_slots <= LORA_SMALL_SLOTS && p.rank * p.n_slices <= LORA_SMALL_RANKS);
   const int64_t ids = p.T < p.n_slots + 1 ? p.T : p.n_slots + 1;
   const int64_t avg = p.T / ids;
   s.rt = s.small || avg < 20 ? 1 : avg < 48 ? 2 : 4;
@@ -434,13 +462,16 @@ LoraShape lora_shape(const ZmiLora &p) {
   // small: K slices of four stages or more while there is less than two workgroups a compute unit
   s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages / 4, 1, 16));
   // planned: a workgroup a compute unit (two share what one already gets through: 512 workgroups 90 us against 82 for 8192
-  // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of eight stages or more
-  s.grid = (int)lora_clamp(s.tiles * s.ny * stages / 8, 8, 256) / 8 * 8;
+  // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of LORA_RUN stages or more (of two up to 128 workgroups)
+  const int64_t all = s.tiles * s.ny * stages, few = lora_clamp(all / 2, 8, 128);
+  s.grid = (int)lora_clamp(all / LORA_RUN, few, 256) / 8 * 8;
   s.terms = p.dt_dst == ZMI_DT_F32 ? 3 : 2;
   s.dma = p.ldx % 8 == 0 && p.a_ld % 8 == 0 && p.a_slot % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
   s.kt = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : p.rank <= 128 ? 4 : 8;
-  // (as many columns as the registers hold B of: k_lora_expand.hip)
-  s.nj = s.kt == 8 ? 2 : s.small || p.dt_x == ZMI_DT_F16 || p.dt_dst == ZMI_DT_F32 ? 4 : 8;
+  // columns of an expand lane: eight, where the registers hold B of so many and every slice's columns are whole eights
+  bool eights = !s.small && p.dt_x == ZMI_DT_BF16 && p.dt_dst != ZMI_DT_F32 && s.kt < 8;
+  for (int i = 0; i < p.n_slices; ++i) eights &= p.N[i] % 8 == 0;
+  s.nj = s.kt == 8 ? 2 : eights ? 8 : 4;
   s.col_blocks = 0;
   const int cols = LORA_WAVES * 16 * s.nj;
   for (int i = 0; i < p.n_slices; ++i) s.col_blocks += (p.N[i] + cols - 1) / cols;
@@ -468,6 +499,7 @@ size_t lora_layout(const ZmiLora &p, const LoraShape &s, char *base, ZmiLoraPlan
     l.h = take((size_t)s.groups * p.n_slices * ((p.rank + 31) / 32) * s.terms * 1024);
     l.partial = (float *)take((size_t)s.grid * 2 * s.rt * s.nt * 1024);
   } else {
+    l.tiles = (int32_t *)take((size_t)s.tiles * 80);
     l.partial = (float *)take((size_t)s.ks * s.tiles * qt * 1024);
   }
   if (w) *w = l;
@@ -519,9 +551,9 @@ hipError_t zmi_launch_lora(const ZmiLora &p, hipStream_t stream, const char **na
   lora_layout(p, s, (char *)p.workspace, &w);
   hipError_t e = hipSuccess;
   if (!s.small) {
-    // (a row of counts per wavefront: 64 KiB of LDS, and a word or two over for the most slots)
-    const int waves = p.n_slots < 1024 ? 16 : p.n_slots < 2048 ? 8 : 4, smem = waves * (p.n_slots + 1) * 4;
-    e = zmi_func_smem_once((const void *)zmi_lora_plan_kernel, 4 * (ZMI_LORA_MAX_SLOTS + 1) * 4);
+    // (a row of counts per wavefront and four words of every slot in LDS)
+    const int waves = p.n_slots < 1024 ? 16 : p.n_slots < 2048 ? 8 : 4, smem = (waves * 4 + 16) * (p.n_slots + 1);
+    e = zmi_func_smem_once((const void *)zmi_lora_plan_kernel, (4 * 4 + 16) * (ZMI_LORA_MAX_SLOTS + 1));
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(zmi_lora_plan_kernel, dim3(1), dim3(1024), smem, stream, p, w, 16 * s.rt, waves);
     e = hipGetLastError();

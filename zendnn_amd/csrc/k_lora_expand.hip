@@ -21,26 +21,34 @@ struct Out {
   static constexpr int COLS = LORA_WAVES * 16 * NJ;   // of a workgroup
   typedef uint32_t run_t __attribute__((ext_vector_type(WORDS)));   // a lane's columns of a row
 
-  // cols < NJ: only that many (edge: some lane of the wavefront has fewer)
-  static __device__ __forceinline__ run_t load(const char *at, int cols, bool edge) {
+  // EDGE: only `cols` of them are there (of some lanes of the wavefront), none where that is not positive; with eight columns
+  // a lane all or none are (the host sees to it)
+  template <bool EDGE>
+  static __device__ __forceinline__ run_t load(const char *at, int cols) {
     run_t y;
-    if (!edge) {
+    if (!EDGE) {
       __builtin_memcpy(&y, at, BYTES);
-    } else {
+    } else if (NJ == 8) {
 #pragma unroll
       for (int k = 0; k < WORDS; ++k) y[k] = 0;
+      if (cols > 0) __builtin_memcpy(&y, at, BYTES);
+    } else {
+      // (the slice's last column in the place of those behind it: no branches, all loads in flight)
+      uint32_t v[NJ];
 #pragma unroll
       for (int e = 0; e < NJ; ++e) {
-        if (e >= cols) continue;
-        if (ES == 4) y[e % WORDS] = ((const uint32_t *)at)[e];
-        else y[e / 2 % WORDS] |= (uint32_t)((const uint16_t *)at)[e] << (16 * (e % 2));
+        const int i = e < cols ? e : cols - 1;
+        v[e] = ES == 4 ? ((const uint32_t *)at)[i] : ((const uint16_t *)at)[i];
       }
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) y[k] = ES == 4 ? v[k % NJ] : v[2 * k % NJ] | v[(2 * k + 1) % NJ] << 16;
     }
     return y;
   }
-  static __device__ __forceinline__ void store(char *at, run_t y, int cols, bool edge) {
-    if (!edge) {
-      __builtin_memcpy(at, &y, BYTES);
+  template <bool EDGE>
+  static __device__ __forceinline__ void store(char *at, run_t y, int cols) {
+    if (!EDGE || NJ == 8) {
+      if (!EDGE || cols > 0) __builtin_memcpy(at, &y, BYTES);
     } else {
 #pragma unroll
       for (int e = 0; e < NJ; ++e) {
@@ -82,14 +90,29 @@ template <bool F16, int NJ, int KT>
 __device__ __forceinline__ void load_b(const ZmiLora &p, int s, int slot, int rank, int n, u32x4 (&b)[KT][NJ][F16 ? 2 : 1]) {
   const int g = threadIdx.x % 64 / 16;
   u32x4 v[KT][NJ];
+  const uint16_t *from[NJ];
 #pragma unroll
-  for (int c = 0; c < KT; ++c)
+  for (int j = 0; j < NJ; ++j) from[j] = (const uint16_t *)p.b[s] + slot * p.b_slot[s] + (n + j < p.N[s] ? n + j : p.N[s] - 1) * p.b_ld[s] + g * 8;
+  // (zeros first, then one masked load each: a second writer of the same registers would have to wait for the first)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int at = n + j < p.N[s] ? n + j : p.N[s] - 1, left = rank - c * 32 - g * 8;
-      const uint16_t *br = (const uint16_t *)p.b[s] + slot * p.b_slot[s] + at * p.b_ld[s] + c * 32 + g * 8;
-      v[c][j] = left >= 8 ? load16(br) : load16_head(br, left);
+  for (int c = 0; c < KT; ++c) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) v[c][j] = u32x4{0, 0, 0, 0};
+    if (rank - c * 32 - g * 8 >= 8) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) v[c][j] = load16(from[j] + c * 32);
     }
+  }
+  if (rank % 8) {
+#pragma unroll
+    for (int c = 0; c < KT; ++c) {
+      const int left = rank - c * 32 - g * 8;
+      if (left > 0 && left < 8) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) v[c][j] = load16_head(from[j] + c * 32, left);
+      }
+    }
+  }
 #pragma unroll
   for (int c = 0; c < KT; ++c)
 #pragma unroll
@@ -151,84 +174,96 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
       asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
                    ::"s"(into + u * 1024), "v"(from + u * 1024) : "memory", "m0");
   };
-  auto load_base = [&](typename O::run_t (&y)[4], int4 rows) {
-    const int row[4] = {rows.x, rows.y, rows.z, rows.w};
+  auto run = [&](auto edge_of) {
+    constexpr bool EDGE = decltype(edge_of)::value;
+    auto load_base = [&](typename O::run_t (&y)[4], int4 rows) {
+      const int row[4] = {rows.x, rows.y, rows.z, rows.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (p.base) y[i] = O::load((const char *)p.base + ((int64_t)(row[i] < 0 ? 0 : row[i]) * p.ld_base + col0 + n) * O::ES, cols, edge);
-      else
+      for (int i = 0; i < 4; ++i) {
+        if (p.base) y[i] = O::template load<EDGE>((const char *)p.base + ((int64_t)(row[i] < 0 ? 0 : row[i]) * p.ld_base + col0 + n) * O::ES, cols);
+        else
 #pragma unroll
-        for (int k = 0; k < O::WORDS; ++k) y[i][k] = 0;
-    }
-  };
-  auto store = [&](const typename O::run_t (&y)[4], int4 rows) {
-    const int row[4] = {rows.x, rows.y, rows.z, rows.w};
+          for (int k = 0; k < O::WORDS; ++k) y[i][k] = 0;
+      }
+    };
+    auto store = [&](const typename O::run_t (&y)[4], int4 rows) {
+      const int row[4] = {rows.x, rows.y, rows.z, rows.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (row[i] >= 0) O::store((char *)p.dst + ((int64_t)row[i] * p.ld_dst + col0 + n) * O::ES, y[i], cols, edge);
-  };
+      for (int i = 0; i < 4; ++i)
+        if (row[i] >= 0) O::template store<EDGE>((char *)p.dst + ((int64_t)row[i] * p.ld_dst + col0 + n) * O::ES, y[i], cols);
+    };
 
-  u32x4 b[KT][NJ][F16 ? 2 : 1];
-  typename O::run_t y[4], y_next[4], out[4];
-  int4 rows = rows_of(a), rows_next = rows_of(a + 1 < z ? a + 1 : a), rows_out = rows;
-  int slot = -1, kts = 0;
-  float scale = 0.0f;
-  send_h(a);
-  if (here) load_base(y, rows);
-  for (int i = a; i < z; ++i) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // all that was asked for one group ago
-    group_barrier();
-    const int4 rows_after = rows_of(i + 2 < z ? i + 2 : z - 1);
-    if (i + 1 < z) {
-      if (here) load_base(y_next, rows_next);
-      send_h(i + 1);
-    }
-    if (here) {
-      if (i > a) store(out, rows_out);
+    u32x4 b[KT][NJ][F16 ? 2 : 1];
+    typename O::run_t y[4], y_next[4], out[4];
+    int4 rows = rows_of(a), rows_next = rows_of(a + 1 < z ? a + 1 : a), rows_out = rows;
+    int slot = -1, kts = 0;
+    float scale = 0.0f;
+    auto take_slot = [&](int i) {
       const int now = __builtin_amdgcn_readfirstlane(w.group_slot[2 * i]);
-      if (now != slot) {
-        slot = now;
-        const int rank = __builtin_amdgcn_readfirstlane(w.group_slot[2 * i + 1]);
-        kts = (rank + 31) / 32;
-        if (kts) {
-          scale = p.scales ? p.scales[slot] : 1.0f;
-          load_b<F16, NJ, KT>(p, s, slot, rank, n, b);
-        }
-      }
-      if (kts) {
-        f32x4 acc[NJ];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < KT; ++c) {
-          if (c >= kts) break;
-#pragma unroll
-          for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, *(const u32x4 *)(ring[i & 1] + (c * TERMS + k) * 1024 + lane * 16), b[c], k + 1 == TERMS);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) out[r] = O::sum(y[r], acc, r, scale);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) out[r] = y[r];
-      }
+      if (now == slot) return;
+      slot = now;
+      const int rank = __builtin_amdgcn_readfirstlane(w.group_slot[2 * i + 1]);
+      kts = (rank + 31) / 32;
+      if (!kts) return;
+      scale = p.scales ? p.scales[slot] : 1.0f;
+      load_b<F16, NJ, KT>(p, s, slot, rank, n, b);
+    };
+    send_h(a);
+    if (here) {
+      load_base(y, rows);
+      take_slot(a);
     }
-    rows_out = rows;
-    rows = rows_next;
-    rows_next = rows_after;
+    for (int i = a; i < z; ++i) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // all that was asked for one group ago
+      group_barrier();
+      const int4 rows_after = rows_of(i + 2 < z ? i + 2 : z - 1);
+      if (i + 1 < z) {
+        if (here) load_base(y_next, rows_next);
+        send_h(i + 1);
+      }
+      if (here) {
+        if (i > a) store(out, rows_out);
+        take_slot(i);
+        if (kts) {
+          f32x4 acc[NJ];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = y_next[r];
-  }
-  if (here) store(out, rows_out);
+          for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < KT; ++c) {
+            if (c >= kts) break;
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, *(const u32x4 *)(ring[i & 1] + (c * TERMS + k) * 1024 + lane * 16), b[c], k + 1 == TERMS);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[r] = O::sum(y[r], acc, r, scale);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[r] = y[r];
+        }
+      }
+      rows_out = rows;
+      rows = rows_next;
+      rows_next = rows_after;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = y_next[r];
+    }
+    if (here) store(out, rows_out);
+  };
+  if (edge) run(std::true_type());   // (the barriers of either are the same ones)
+  else run(std::false_type());
 }
 
-// Up to 64 rows: workgroup (x: columns of a slice, y: tile of up to 16 rows); h comes as the K slices' sums.
+// Up to 128 rows: workgroup (x: columns of a slice, y: tile of up to 16 rows); h comes as the K slices' sums.
 template <bool F16, int NJ, int KT, int DST>
 __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_small_kernel(ZmiLora p, ZmiLoraPlan w, int slices) {
   typedef Out<NJ, DST> O;
   constexpr int TERMS = O::TERMS;
   const int lane = threadIdx.x % 64, g = lane / 16, c16 = lane % 16;
-  Tile t;
-  if (!lora_find_tile(p, blockIdx.y, t)) return;
+  // the tile as the shrink launch found it
+  const int32_t *entry = w.tiles + blockIdx.y * 20;
+  const int4 e = *(const int4 *)entry, rows = *(const int4 *)(entry + 4 + g * 4);
+  const int slot = __builtin_amdgcn_readfirstlane(e.x), count = __builtin_amdgcn_readfirstlane(e.y), rank = __builtin_amdgcn_readfirstlane(e.z);
+  if (!count) return;
   int s = 0, blk = blockIdx.x, col0 = 0;
   while (blk >= (p.N[s] + O::COLS - 1) / O::COLS) {
     blk -= (p.N[s] + O::COLS - 1) / O::COLS;
@@ -236,69 +271,93 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_small_kern
   }
   const int n0 = blk * O::COLS + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 16 * NJ;
   if (n0 >= p.N[s]) return;
-  const bool none = t.slot == p.n_slots, edge = n0 + 16 * NJ > p.N[s];
+  const bool none = slot == p.n_slots, edge = n0 + 16 * NJ > p.N[s];
   if (none && p.base == p.dst) return;
   const int n = n0 + c16 * NJ, cols = p.N[s] - n;
-  int64_t row[4];
-  typename O::run_t y[4];
+  const int row[4] = {rows.x, rows.y, rows.z, rows.w};
+  auto run = [&](auto edge_of) {
+    constexpr bool EDGE = decltype(edge_of)::value;
+    typename O::run_t y[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = g * 4 + i;
-    row[i] = __shfl(t.row, at < t.n ? at : 0, 64);
-    if (p.base) y[i] = O::load((const char *)p.base + (row[i] * p.ld_base + col0 + n) * O::ES, cols, edge);
-    else
+    for (int i = 0; i < 4; ++i) {
+      if (p.base) y[i] = O::template load<EDGE>((const char *)p.base + ((int64_t)(row[i] < 0 ? 0 : row[i]) * p.ld_base + col0 + n) * O::ES, cols);
+      else
 #pragma unroll
-      for (int k = 0; k < O::WORDS; ++k) y[i][k] = 0;
-  }
-  if (!none) {
-    const int rank = lora_rank(p, t.slot), kts = (rank + 31) / 32, lt = (rank + 15) / 16, qt = p.n_slices * ((p.rank + 15) / 16);
-    const float scale = p.scales ? p.scales[t.slot] : 1.0f;
-    u32x4 b[KT][NJ][F16 ? 2 : 1];
-    load_b<F16, NJ, KT>(p, s, t.slot, rank, n, b);
-    f32x4 acc[NJ];
+        for (int k = 0; k < O::WORDS; ++k) y[i][k] = 0;
+    }
+    if (!none) {
+      const int kts = (rank + 31) / 32, lt = (rank + 15) / 16, qt = p.n_slices * ((p.rank + 15) / 16);
+      const float scale = p.scales ? p.scales[slot] : 1.0f;
+      u32x4 b[KT][NJ][F16 ? 2 : 1];
+      load_b<F16, NJ, KT>(p, s, slot, rank, n, b);
+      f32x4 acc[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
+      for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int c = 0; c < KT; ++c) {
-      if (c >= kts) break;
-      // ranks (r % 16 / 4) * 16 + row, four to a lane
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      const int r = c * 32 + g * 8, left = rank - r;
-      if (left > 0 && c16 < t.n) {
-        for (int k = 0; k < slices; ++k) {
-          const int64_t at = ((int64_t)k * gridDim.y + blockIdx.y) * qt + s * lt + r / 16;
-          const f32x4 *src = (const f32x4 *)w.partial + at * 64 + r % 16 / 4 * 16 + c16;
-          const f32x4 lo = src[0], hi = src[16];
+      for (int c = 0; c < KT; ++c) {
+        if (c >= kts) break;
+        // ranks (r % 16 / 4) * 16 + row, four to a lane
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const int r = c * 32 + g * 8, left = rank - r;
+        if (left > 0 && c16 < count) {
+          const f32x4 *src = (const f32x4 *)w.partial + ((int64_t)blockIdx.y * qt + s * lt + r / 16) * 64 + r % 16 / 4 * 16 + c16;
+          const int64_t step = (int64_t)gridDim.y * qt * 64;
+          for (int k0 = 0; k0 < slices; k0 += 4) {   // (four slices' sums in flight)
+            f32x4 part[4][2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[4 + e] += hi[e]; }
+            for (int k = 0; k < 4; ++k) {
+              const f32x4 *at = src + (k0 + k < slices ? k0 + k : k0) * step;
+              part[k][0] = at[0];
+              part[k][1] = at[16];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] += k0 + k < slices ? part[k][0][e] : 0.0f;
+                v[4 + e] += k0 + k < slices ? part[k][1][e] : 0.0f;
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e >= left) v[e] = 0.0f;
         }
+        __bf16 h[TERMS][8];
+        split<TERMS>(v, h);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e >= left) v[e] = 0.0f;
+        for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, pack8(h[k]), b[c], k + 1 == TERMS);
       }
-      __bf16 h[TERMS][8];
-      split<TERMS>(v, h);
+      if (kts) {
 #pragma unroll
-      for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, pack8(h[k]), b[c], k + 1 == TERMS);
+        for (int i = 0; i < 4; ++i) y[i] = O::sum(y[i], acc, i, scale);
+      }
     }
-    if (kts) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = O::sum(y[i], acc, i, scale);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (g * 4 + i < t.n) O::store((char *)p.dst + (row[i] * p.ld_dst + col0 + n) * O::ES, y[i], cols, edge);
+    for (int i = 0; i < 4; ++i)
+      if (row[i] >= 0) O::template store<EDGE>((char *)p.dst + ((int64_t)row[i] * p.ld_dst + col0 + n) * O::ES, y[i], cols);
+  };
+  if (edge) run(std::true_type());
+  else run(std::false_type());
 }
 
 namespace {
 
 template <bool F16, int KT, int DST>
 void launch_as(const ZmiLora &p, const ZmiLoraPlan &w, const LoraShape &s, hipStream_t stream) {
-  constexpr int FEW = KT == 8 ? 2 : 4, NJ = F16 || KT == 8 || DST == ZMI_DT_F32 ? FEW : 8;
+  constexpr int FEW = KT == 8 ? 2 : 4;
   const dim3 block(LORA_WAVES * 64);
-  if (s.small) hipLaunchKernelGGL((zmi_lora_expand_small_kernel<F16, FEW, KT, DST>), dim3((unsigned)s.col_blocks, (unsigned)s.tiles), block, 0, stream, p, w, s.ks);
-  else hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, NJ, KT, DST>), dim3((unsigned)s.col_blocks, (unsigned)s.runs), block, 0, stream, p, w);
+  if (s.small) {
+    hipLaunchKernelGGL((zmi_lora_expand_small_kernel<F16, FEW, KT, DST>), dim3((unsigned)s.col_blocks, (unsigned)s.tiles), block, 0, stream, p, w, s.ks);
+    return;
+  }
+  const dim3 grid((unsigned)s.col_blocks, (unsigned)s.runs);
+  if constexpr (!F16 && KT < 8 && DST != ZMI_DT_F32) {
+    if (s.nj == 8) {
+      hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, 8, KT, DST>), grid, block, 0, stream, p, w);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, FEW, KT, DST>), grid, block, 0, stream, p, w);
 }
 
 template <bool F16, int KT>

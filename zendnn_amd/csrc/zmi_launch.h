@@ -349,7 +349,7 @@ struct ZmiLora {
 // the parts of the workspace
 struct ZmiLoraPlan {
   int32_t *header;            // number of tiles, of 16-row groups with an adapter, of all groups
-  int32_t *tiles;             // {slot, number of its first group, rows, rank} of each shrink tile
+  int32_t *tiles;             // {slot, number of its first group, rows, rank} of each shrink tile (small calls: see k_lora.hip)
   int32_t *group_slot;        // {slot, rank} of each group
   int32_t *order;             // the groups' rows, 16 each, -1: none
   int32_t *place;             // (the plan launch's own)

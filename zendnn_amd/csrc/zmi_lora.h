@@ -4,7 +4,12 @@
 #include "zmi_launch.h"
 
 #define LORA_WAVES 4
-#define LORA_SMALL_T 64     // rows up to which wavefronts plan for themselves
+// Rows up to which wavefronts plan for themselves: any slots, or few slots and ranks (a round of the search per distinct slot,
+// and a tile's 16 rows read all of their slot's A and B)
+#define LORA_SMALL_T 128
+#define LORA_SMALL_MOST 512
+#define LORA_SMALL_SLOTS 16
+#define LORA_SMALL_RANKS 64
 
 // How a call goes out (k_lora.hip: lora_shape)
 struct LoraShape {
@@ -39,13 +44,14 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x4 load16(const void *p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
 __device__ __forceinline__ void store16(void *p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
 
-// the first n (< 8) of eight 16-bit elements, zeros behind them
+// the first n (1 .. 7) of eight 16-bit elements, zeros behind them: four, two and one, as n has them
 __device__ __forceinline__ u32x4 load16_head(const uint16_t *p, int n) {
-  u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) v[i / 2] |= (uint32_t)p[i] << (16 * (i % 2));
-  return v;
+  uint32_t four[2] = {0, 0}, two = 0, one = 0;
+  if (n & 4) __builtin_memcpy(four, p, 8);
+  if (n & 2) __builtin_memcpy(&two, p + (n & 4), 4);
+  if (n & 1) one = p[n & 6];
+  const uint32_t lo = n & 2 ? two : one, hi = n & 2 ? one : 0;
+  return n & 4 ? u32x4{four[0], four[1], lo, hi} : u32x4{lo, hi, 0, 0};
 }
 
 __device__ __forceinline__ int lora_rank(const ZmiLora &p, int slot) {
@@ -61,36 +67,120 @@ struct Tile {
   int row;    // unplanned: lane l's row is that of position l % 16
 };
 
-// Tile `want` of up to 64 rows: slots in the order of their first rows, 16 rows each.
-__device__ __forceinline__ bool lora_find_tile(const ZmiLora &p, int want, Tile &t) {
+// The tile of rows `sub` * 16 .. +15 among the c rows of a slot, whose lanes (row 64 h + lane) are m[h].
+template <int H>
+__device__ __forceinline__ void lora_tile_rows(const uint64_t (&m)[H], int c, int slot, int sub, Tile &t) {
   const int lane = threadIdx.x % 64;
-  int id = -1;
-  if (lane < p.T) {
-    id = p.slot_ids[lane];
-    if ((unsigned)id >= (unsigned)p.n_slots) id = p.n_slots;
+  int got = 0, before = 0;
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const int pos = before + __popcll(m[h] & ((1ull << lane) - 1));
+    const bool in = ((m[h] >> lane) & 1) && pos / 16 == sub;
+    // (lanes outside push to the upper lanes, which nobody reads; a lane that nothing is pushed to gets 0)
+    const int row = __builtin_amdgcn_ds_permute(4 * (in ? pos % 16 : 16 + lane % 48), in ? lane + 64 * h + 1 : 0);
+    got = row > got ? row : got;
+    before += __popcll(m[h]);
   }
-  uint64_t left = __ballot(lane < p.T);
+  t.slot = slot;
+  t.n = c - 16 * sub < 16 ? c - 16 * sub : 16;
+  t.group = 0;
+  t.row = __shfl(got, lane % 16, 64) - 1;
+}
+
+// Tile `want` of up to 64 H rows: slots in the order of their first rows, 16 rows each; a round per distinct id.
+template <int H>
+__device__ __forceinline__ bool lora_find_tile_few_slots(const ZmiLora &p, int want, Tile &t) {
+  const int lane = threadIdx.x % 64, parts = (p.T + 63) / 64;
+  int id[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) id[h] = h < parts ? p.slot_ids[lane + 64 * h < p.T ? lane + 64 * h : p.T - 1] : 0;
+  uint64_t left[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    if ((unsigned)id[h] >= (unsigned)p.n_slots) id[h] = p.n_slots;
+    left[h] = __ballot(lane + 64 * h < p.T);
+  }
   int seen = 0;
-  while (left) {
-    const int slot = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    const uint64_t m = __ballot(id == slot);
-    const int c = __popcll(m), tiles = (c + 15) / 16;
+  for (;;) {
+    int slot = -1;
+#pragma unroll
+    for (int h = H - 1; h >= 0; --h)
+      if (left[h]) slot = __builtin_amdgcn_readlane(id[h], __builtin_ctzll(left[h]));
+    if (slot < 0) return false;
+    uint64_t m[H];
+    int c = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      m[h] = h < parts ? __ballot(id[h] == slot) & left[h] : 0;
+      c += __popcll(m[h]);
+    }
+    const int tiles = (c + 15) / 16;
     if (want < seen + tiles) {
-      const int sub = want - seen;
-      const int pos = __popcll(m & ((1ull << lane) - 1));
-      const bool in = id == slot && pos / 16 == sub;
-      // (lanes outside push to the upper lanes, which nobody reads)
-      const int got = __builtin_amdgcn_ds_permute(4 * (in ? pos % 16 : 63), lane);
-      t.slot = slot;
-      t.n = c - 16 * sub < 16 ? c - 16 * sub : 16;
-      t.group = 0;
-      t.row = __shfl(got, lane % 16, 64);
+      lora_tile_rows<H>(m, c, slot, want - seen, t);
       return true;
     }
     seen += tiles;
-    left &= ~m;
+#pragma unroll
+    for (int h = 0; h < H; ++h) left[h] &= ~m[h];
+  }
+}
+
+// The same of up to 128 rows, without the rounds: every lane finds the rows that share its slot bit by bit, the first of
+// them counts their tiles, and a running sum over the lanes says whose tile it is.
+__device__ __forceinline__ bool lora_find_tile_few_rows(const ZmiLora &p, int want, Tile &t) {
+  const int lane = threadIdx.x % 64;
+  const uint64_t below = (1ull << lane) - 1;
+  int id[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) id[h] = p.slot_ids[lane + 64 * h < p.T ? lane + 64 * h : p.T - 1];
+  uint64_t m[2][2];   // [this lane's row of half h][rows of half g that share its slot]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if ((unsigned)id[h] >= (unsigned)p.n_slots) id[h] = p.n_slots;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) m[h][g] = __ballot(lane + 64 * g < p.T);
+  }
+  const int bits = 32 - __builtin_clz(p.n_slots);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t one[2] = {__ballot((id[0] >> b) & 1), __ballot((id[1] >> b) & 1)};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) m[h][g] &= (id[h] >> b) & 1 ? one[g] : ~one[g];
+  }
+  int c[2], tiles[2], end[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    c[h] = __popcll(m[h][0]) + __popcll(m[h][1]);
+    const bool first = lane + 64 * h < p.T && !(m[h][h] & below) && (h == 0 || !m[h][0]);
+    tiles[h] = first ? (c[h] + 15) / 16 : 0;
+    end[h] = tiles[h];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(end[h], d, 64);
+      if (lane >= d) end[h] += v;
+    }
+  }
+  end[1] += __builtin_amdgcn_readlane(end[0], 63);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t hit = __ballot(want < end[h] && want >= end[h] - tiles[h]);
+    if (!hit) continue;
+    const int at = __builtin_ctzll(hit);
+    uint64_t mine[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+      mine[g] = (uint32_t)__builtin_amdgcn_readlane((int)m[h][g], at) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m[h][g] >> 32), at) << 32;
+    lora_tile_rows<2>(mine, __builtin_amdgcn_readlane(c[h], at), __builtin_amdgcn_readlane(id[h], at),
+                      want - __builtin_amdgcn_readlane(end[h] - tiles[h], at), t);
+    return true;
   }
   return false;
+}
+
+__device__ __forceinline__ bool lora_find_tile(const ZmiLora &p, int want, Tile &t) {
+  if (p.T > 128) return lora_find_tile_few_slots<LORA_SMALL_MOST / 64>(p, want, t);
+  return p.n_slots <= LORA_SMALL_SLOTS ? lora_find_tile_few_slots<2>(p, want, t) : lora_find_tile_few_rows(p, want, t);
 }
 
 template <bool F16>
