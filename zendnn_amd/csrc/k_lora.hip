@@ -451,13 +451,18 @@ LoraShape lora_shape(const ZmiLora &p) {
   LoraShape s = {};
   s.small = p.T <= LORA_SMALL_T || (p.T <= LORA_SMALL_MOST && p.n_slots <= LORA_SMALL_SLOTS && p.rank * p.n_slices <= LORA_SMALL_RANKS);
   const int64_t ids = p.T < p.n_slots + 1 ? p.T : p.n_slots + 1;
-  const int64_t avg = p.T / ids;
-  s.rt = s.small || avg < 20 ? 1 : avg < 48 ? 2 : 4;
-  s.tiles = ids + (p.T - ids) / (16 * s.rt);
-  s.groups = ids + (p.T - ids) / 16;
   const int qt = p.n_slices * ((p.rank + 15) / 16);
   s.nt = qt >= 8 ? 8 : qt > 2 ? 4 : qt;
   s.ny = (qt + s.nt - 1) / s.nt;
+  // Tall tiles read A less often, low ones leave fewer pieces of a tile to join: half as many row groups as rank tiles, more
+  // while there are two tiles a workgroup, and no more than the slots' rows fill on average (2048 rows of K = 4096, 1 / 2 / 4
+  // groups: rank 8 8.1 / 9.0 / 11.2 us, rank 64 15.1 / 12.9 / 15.5; 8192 rows of K = 14336, rank 128: 132 / 95 / 78).
+  const int64_t avg = p.T / ids;
+  const int most = s.small || avg < 20 ? 1 : avg < 48 ? 2 : 4;
+  s.rt = s.nt / 2 < 1 ? 1 : s.nt / 2 < most ? s.nt / 2 : most;
+  while (s.rt < most && p.T / (32 * s.rt) * s.ny >= 512) s.rt *= 2;
+  s.tiles = ids + (p.T - ids) / (16 * s.rt);
+  s.groups = ids + (p.T - ids) / 16;
   const int64_t stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
   // small: K slices of four stages or more while there is less than two workgroups a compute unit
   s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages / 4, 1, 16));
