@@ -54,7 +54,7 @@ class Case:
         """(exact result, tolerance) in float64."""
         y = base.double() if base is not None else torch.zeros(self.T, sum(self.N), dtype=torch.float64, device=H.DEV)
         tol = torch.zeros_like(y)
-        for s in range(self.S):
+        for s in sorted({int(i) for i in self.ids.tolist() if 0 <= i < self.S}):
             rows = (self.ids == s).nonzero()[:, 0]
             r = min(max(int(self.ranks[s]), 0), self.rank) if self.ranks is not None else self.rank
             if not len(rows) or not r:
@@ -327,3 +327,23 @@ def test_wrappers_refuse_what_they_cannot_describe():
         args = dict(x=c.x, slot_ids=c.ids, a=c.a, b=c.b[0], dst=c.dst) | kw
         with pytest.raises(ValueError):
             lowoha.lora_direct(**args)
+
+
+@pytest.mark.parametrize("T,K,N,rank,S", [(129, 256, [96], 8, 17), (512, 320, [72, 40], 16, 16), (513, 320, [72, 40], 16, 16), (512, 320, [72], 33, 2),
+                                          (500, 64, [16], 8, 4096), (5000, 72, [24], 8, 4095), (9001, 128, [40], 16, 7), (20000, 64, [16], 4, 1500),
+                                          (33000, 64, [8], 8, 2), (4097, 4096, [64], 8, 3), (3000, 1024, [64], 200, 6), (700, 2048, [128, 64, 64], 256, 2)])
+def test_plans(T, K, N, rank, S):
+    """Batches on both sides of the borders between the ways of sorting rows: few and many rows, slots and ranks."""
+    c = Case(T + S, T, K, N, rank, S, mixed=S < 100)
+    c.check("other")
+    c.check("dst")
+    first = c.call(c.base, dst=c.dst) == capi.SUCCESS and c.dst.clone()
+    assert c.call(c.base) == capi.SUCCESS and torch.equal(first, c.dst)
+
+
+def test_sorted_batches_and_long_runs():
+    """Rows of a request next to each other, and one request that fills the batch."""
+    for T in (300, 3000):
+        i32 = dict(dtype=torch.int32, device=H.DEV)
+        for ids in ((torch.arange(T, **i32) * 5 // T), torch.zeros(T, **i32), torch.arange(T, **i32).flip(0) * 6 // T - 1):
+            Case(T, T, 1024, [264], 32, 5, ids=ids.contiguous()).check("dst")
