@@ -395,7 +395,7 @@ ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
  * workspace: device memory of zmi_lora_workspace_size() bytes, 16-byte aligned; null: the calling thread's scratch
  * arena, which a stream that is being captured into a graph cannot use (failure) -- give a captured call a workspace that
  * no other graph shares.  T == 0 is an empty batch: success.
- * Limits: rank <= 256, n_slices <= ZMI_LORA_MAX_SLICES, n_slots <= 4096, T <= 2^20, K <= 2^19. */
+ * Limits: rank <= 256, n_slices <= ZMI_LORA_MAX_SLICES, n_slots <= 4096, T <= 2^20, K <= 2^19, 2^30 columns. */
 #define ZMI_LORA_MAX_SLICES 4
 typedef struct zmi_lora_t {
   int32_t T, K, rank, n_slices, n_slots;

@@ -1,9 +1,11 @@
 """GPU tests of zmi_moe_router_grouped (through the C ABI): ids bit-exact and weights to 1e-6 relative against the
 definition in float64 on the host.
 
-The weights' tolerance: the score of a chosen expert is an exponential (3 ulp in f32) over a sum of at most 512 such
-terms (3 ulp each, at most 10 roundings on the way), divided by a sum of at most 64 scores: fewer than 16 half steps of
-2^-24 = 9.5e-7 even if everything were computed in f32."""
+The weights' tolerance, in half steps of 2^-24: a score's exponential is within 2 ulp (4 half steps), the terms of a
+softmax's sum are too, and a lane adds up to eight of them in f32, three roundings deep (7 together); sums over lanes and
+over the chosen, the division and the scale are in 64 bits, and the result is rounded once: 4 + 7 + 1 = 12 half steps,
+7.2e-7.
+"""
 import numpy as np
 import pytest
 import torch

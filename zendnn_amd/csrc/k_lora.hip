@@ -75,6 +75,7 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
       // (LDS serves a wavefront in order: everybody has read before the last lane of each slot writes)
       if (same >> lane == 1) mine[slot] = at + 1;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (other lanes' writes are read by the next 64 rows)
     return at;
   };
 #pragma unroll
@@ -160,11 +161,16 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
 //
 // K goes through an LDS ring of D stages of KS elements: x rows and A rows alike are moved in units of 8 rows x 128
 // bytes, one 16-byte piece a lane.  (MFMA operands read from global memory directly put 16 rows under 16 neighbouring
-// lanes: every 16 bytes a cache line of its own, and the compute unit's address path, not HBM, sets the pace: 148 us for
-// 8192 rows of K = 14336 at rank 128 against 62 us through LDS.)  Piece c of row r stands at slot c ^ (r % 8), which
+// lanes: every 16 bytes an access of its own, and the compute unit's address path, not HBM, sets the pace: 148 us for
+// 8192 rows of K = 14336 at rank 128 against 78 us through LDS.)  Piece c of row r stands at slot c ^ (r % 8), which
 // spreads the operand reads over the banks.  With rows, strides and addresses of 16-byte multiples the units are moved
 // by global -> LDS loads (DMA), D - 1 stages ahead; otherwise through registers, one stage ahead.
 // The four wavefronts share a stage as WR x WN x WK over row groups, rank tiles and 64-element blocks of K.
+//
+// What bounds it: the cache lines a compute unit can have outstanding (about 90: the sum of all read latencies over the
+// launch's time), 16 clocks a line of x from HBM and 6 a line of A from L2.  206 MB of x and 0.3 GB of A from L2 in the 78 us
+// above, 4.9 TB/s from HBM and L2 together a compute unit's share of 21 bytes a clock; without its arithmetic the launch
+// takes the same time, without its loads 52 us.
 // ---------------------------------------------------------------------------------------------------------------
 template <bool F16, int RT, int NT, int KS, int WR, int WN, int D, bool DMA, bool SMALL>
 __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(ZmiLora p, ZmiLoraPlan w, int ny) {
@@ -464,10 +470,12 @@ LoraShape lora_shape(const ZmiLora &p) {
   s.tiles = ids + (p.T - ids) / (16 * s.rt);
   s.groups = ids + (p.T - ids) / 16;
   const int64_t stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
-  // small: K slices of four stages or more while there is less than two workgroups a compute unit
+  // small: K slices of four stages or more while there are less than two workgroups a compute unit (48 rows, 64 slots, three
+  // slices of rank 64, both launches: 256 workgroups 23.8 us, 512 22.4, 1024 28.5)
   s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages / 4, 1, 16));
   // planned: a workgroup a compute unit (two share what one already gets through: 512 workgroups 90 us against 82 for 8192
-  // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of LORA_RUN stages or more (of two up to 128 workgroups)
+  // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of LORA_RUN stages or more (of two up
+  // to 128 workgroups)
   const int64_t all = s.tiles * s.ny * stages, few = lora_clamp(all / 2, 8, 128);
   s.grid = (int)lora_clamp(all / LORA_RUN, few, 256) / 8 * 8;
   s.terms = p.dt_dst == ZMI_DT_F32 ? 3 : 2;

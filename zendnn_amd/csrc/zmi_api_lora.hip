@@ -18,7 +18,7 @@ int32_t lora_check_sizes(const zmi_lora_t &l) {
     if (l.N[s] <= 0) { set_error("lora: bad sizes"); return ZMI_FAILURE; }
     cols += l.N[s];
   }
-  if (cols > 0x7fffff00) { set_error("lora: too many columns"); return ZMI_UNIMPLEMENTED; }
+  if (cols > 1 << 30) { set_error("lora: too many columns"); return ZMI_UNIMPLEMENTED; }
   // (tiles x rank tile sets x stages of K stay below 2^31: 20.5 k x 8 x 8192)
   if (l.T > 1 << 20 || l.K > 1 << 19) { set_error("lora: at most 2^20 rows, K at most 2^19"); return ZMI_UNIMPLEMENTED; }
   if (!half_type(l.dt_x)) { set_error("lora: dt_x must be bf16 or f16"); return ZMI_UNIMPLEMENTED; }
