@@ -109,20 +109,17 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
   int start[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    int v = sums[k];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(v, d, 64);
-      if (lane >= d) v += o;
-    }
+    const int v = lora_running_sum(sums[k]);
     if (lane == 63) wave_sums[k][wave] = v;
     start[k] = v - sums[k];
   }
-  __syncthreads();
+  if (n > 64) {   // (else the first wavefront has all slots)
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 16; ++i)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) start[k] += i < wave ? wave_sums[k][i] : 0;
+      for (int k = 0; k < 2; ++k) start[k] += i < wave ? wave_sums[k][i] : 0;
+  }
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     const int i = tid * per + k;

@@ -60,6 +60,19 @@ __device__ __forceinline__ int lora_rank(const ZmiLora &p, int slot) {
   return r < 0 ? 0 : r > p.rank ? p.rank : r;
 }
 
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int lora_dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+// sum over the lanes up to this one
+__device__ __forceinline__ int lora_running_sum(int v) {
+  v += lora_dpp<0x111>(v);        // row_shr 1, 2, 4, 8: inside rows of 16
+  v += lora_dpp<0x112>(v);
+  v += lora_dpp<0x114>(v);
+  v += lora_dpp<0x118>(v);
+  v += lora_dpp<0x142, 0xa>(v);   // row_bcast 15 into rows 1 and 3
+  v += lora_dpp<0x143, 0xc>(v);   // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
 struct Tile {
   int slot;   // n_slots: rows without an adapter
   int n;      // rows of the tile
@@ -154,12 +167,7 @@ __device__ __forceinline__ bool lora_find_tile_few_rows(const ZmiLora &p, int wa
     c[h] = __popcll(m[h][0]) + __popcll(m[h][1]);
     const bool first = lane + 64 * h < p.T && !(m[h][h] & below) && (h == 0 || !m[h][0]);
     tiles[h] = first ? (c[h] + 15) / 16 : 0;
-    end[h] = tiles[h];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(end[h], d, 64);
-      if (lane >= d) end[h] += v;
-    }
+    end[h] = lora_running_sum(tiles[h]);
   }
   end[1] += __builtin_amdgcn_readlane(end[0], 63);
 #pragma unroll
