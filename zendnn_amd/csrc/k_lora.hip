@@ -455,7 +455,9 @@ LoraShape lora_shape(const ZmiLora &p) {
   s.small = p.T <= LORA_SMALL_T || (p.T <= LORA_SMALL_MOST && p.n_slots <= LORA_SMALL_SLOTS && p.rank * p.n_slices <= LORA_SMALL_RANKS);
   const int64_t ids = p.T < p.n_slots + 1 ? p.T : p.n_slots + 1;
   const int qt = p.n_slices * ((p.rank + 15) / 16);
-  s.nt = qt >= 8 ? 8 : qt > 2 ? 4 : qt;
+  // (small calls: four rank tiles fit the live ones of a smaller adapter better, and take fewer K slices: 48 rows, three slices
+  // of rank 64, both launches 22.2 us with eight, 20.8 with four)
+  s.nt = qt >= 8 && !s.small ? 8 : qt > 2 ? 4 : qt;
   s.ny = (qt + s.nt - 1) / s.nt;
   // Tall tiles read A less often, low ones leave fewer pieces of a tile to join: half as many row groups as rank tiles, more
   // while there are two tiles a workgroup, and no more than the slots' rows fill on average (2048 rows of K = 4096, 1 / 2 / 4
@@ -467,9 +469,10 @@ LoraShape lora_shape(const ZmiLora &p) {
   s.tiles = ids + (p.T - ids) / (16 * s.rt);
   s.groups = ids + (p.T - ids) / 16;
   const int64_t stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
-  // small: K slices of four stages or more while there are less than two workgroups a compute unit (48 rows, 64 slots, three
-  // slices of rank 64, both launches: 256 workgroups 23.8 us, 512 22.4, 1024 28.5)
-  s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages / 4, 1, 16));
+  // small: K slices of four stages or more (of one where K has few: 301 rows of K = 1001 7.6 us in four slices, 8.6 in one)
+  // while there are less than two workgroups a compute unit (48 rows, 64 slots, three
+  // slices of rank 64 in eights of rank tiles, both launches: 256 workgroups 23.8 us, 512 22.4, 1024 28.5)
+  s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages >= 16 ? stages / 4 : stages, 1, 16));
   // planned: a workgroup a compute unit (two share what one already gets through: 512 workgroups 90 us against 82 for 8192
   // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of LORA_RUN stages or more (of two up
   // to 128 workgroups)

@@ -80,18 +80,18 @@ __device__ __forceinline__ uint64_t rgk_key(double x) {
 __device__ __forceinline__ float rgk_value(uint32_t k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ double rgk_value(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k)); }
 
-// A lane's J keys in descending order, equal ones in ascending j (neighbours are exchanged only when out of order);
-// returns the j of each, four bits apiece, the first in the lowest bits.
-template <int J, class K>
+// The DEPTH largest of a lane's J keys in descending order, equal ones in ascending j (neighbours are exchanged only when out
+// of order); returns the j of each, four bits apiece, the first in the lowest bits, and ones behind them.
+template <int J, int DEPTH, class K>
 __device__ __forceinline__ uint32_t rgk_sort(K (&key)[J]) {
   // (a vector, not an array: choosing between two elements of an array becomes an indexed read, a chain of comparisons)
   typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
   u32x8 at = {0, 1, 2, 3, 4, 5, 6, 7};
-  uint32_t queue = 0;
+  uint32_t queue = DEPTH < 8 ? ~0u << (4 * DEPTH % 32) : 0u;
 #pragma unroll
-  for (int r = 0; r < J; ++r)
+  for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
-    for (int j = r % 2; j + 1 < J; j += 2) {
+    for (int j = J - 2; j >= d; --j) {
       const bool swap = key[j + 1] > key[j];
       const K hi = max(key[j], key[j + 1]), lo = min(key[j], key[j + 1]);
       const uint32_t a = at[j], b = at[j + 1];
@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t rgk_sort(K (&key)[J]) {
       at[j + 1] = swap ? a : b;
     }
 #pragma unroll
-  for (int j = 0; j < J; ++j) queue |= at[j] << (4 * j);
+  for (int j = 0; j < DEPTH; ++j) queue |= at[j] << (4 * j);
   return queue;
 }
 
@@ -175,8 +175,10 @@ __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J
       if (j < n && !((groups >> of) & 1u)) key[j] = 0;
     }
   }
-  // rounds: the largest first key of a lane, of the lowest lane that has it
-  uint32_t queue = rgk_sort<J>(key);
+  // rounds: the largest first key of a lane, of the lowest lane that has it.  Of eight experts a lane sorts three: that a lane
+  // has to give more happens to one token in some thousands, which is then chosen again from whole lanes.
+  constexpr int DEPTH = std::is_same<V, float>::value && J > 4 ? 3 : J;
+  uint32_t queue = rgk_sort<J, DEPTH>(key);
   uint32_t order = 0;   // float values: lane r keeps the r-th key
   for (int r = 0; r < p.topk; ++r) {
     const K top = rgk_wave_max(key[0]);
@@ -185,11 +187,12 @@ __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J
     if (lane == r) { *mine = e; order = (uint32_t)top; }
     if (lane == at) {
 #pragma unroll
-      for (int j = 0; j + 1 < J; ++j) key[j] = key[j + 1];
-      key[J - 1] = 0;
-      queue >>= 4;
+      for (int j = 0; j + 1 < DEPTH; ++j) key[j] = key[j + 1];
+      key[DEPTH - 1] = 0;
+      queue = DEPTH < 8 ? (uint32_t)((int32_t)queue >> 4) : queue >> 4;
     }
   }
+  if (DEPTH < J && __ballot((queue & 15) == 15)) return false;
   if (std::is_same<V, float>::value && p.bias) {
     const uint32_t rest = (uint32_t)rgk_wave_max(key[0]), below = (uint32_t)__shfl_down((int)order, 1, 64);
     const uint32_t next = lane == p.topk - 1 ? rest : below;
