@@ -359,7 +359,7 @@ ZMI_API int32_t zmi_moe_router_topk(const void *logits, int32_t logits_dt, int64
  *            zeros), times scale.  A NaN logit makes the weights that it enters NaN.
  * Without a bias and groups valued by their sum the order is the logits' own, so scores that round to one value are
  * still told apart.  T == 0 is an empty batch: success.
- * Limits: E <= 512, E a multiple of n_group, n_group <= 64, topk <= min(64, topk_group * E / n_group);
+ * Limits: T <= 2^25, E <= 512, E a multiple of n_group, n_group <= 64, topk <= min(64, topk_group * E / n_group);
  * ZMI_GROUP_TOP2_SUM needs groups of two experts or more. */
 enum zmi_router_scoring { ZMI_SCORE_SOFTMAX = 0, ZMI_SCORE_SIGMOID = 1 };
 enum zmi_router_group_score { ZMI_GROUP_MAX = 0, ZMI_GROUP_TOP2_SUM = 1 };

@@ -124,3 +124,12 @@ def test_python_wrappers_refuse_tensors_they_cannot_describe():
         lowoha.lora_direct(x.float(), torch.zeros(4, dtype=torch.int32), x, x, x)
     with pytest.raises(ValueError, match="slices"):
         lowoha.lora_direct(x, torch.zeros(4, dtype=torch.int32), x, [], x)
+
+
+@fake_pointers
+def test_router_batches_longer_than_a_launch_are_refused():
+    for T in ((1 << 25) + 1, 0x7fffffff):
+        st, err = router(T=T)
+        assert st == capi.UNIMPLEMENTED and "2^25" in err
+    st, err = router(T=1 << 25)
+    assert st == capi.FAILURE and "64 KiB" in err

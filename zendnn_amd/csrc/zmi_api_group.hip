@@ -852,6 +852,7 @@ int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r) {
   clear_error();
   if (!r || r->T < 0 || r->E <= 0 || r->topk <= 0 || r->ldl < r->E || r->n_group <= 0) { set_error("moe_router_grouped: bad arguments"); return ZMI_FAILURE; }
   if (r->E > 512 || r->topk > 64 || r->n_group > 64) { set_error("moe_router_grouped: at most 512 experts, 64 groups and topk <= 64"); return ZMI_UNIMPLEMENTED; }
+  if (r->T > 1 << 25) { set_error("moe_router_grouped: at most 2^25 tokens"); return ZMI_UNIMPLEMENTED; }   // (a launch has less than 2^32 threads)
   if (r->E % r->n_group) { set_error("moe_router_grouped: the groups must divide the experts"); return ZMI_FAILURE; }
   const int per = r->E / r->n_group;
   if (r->topk_group <= 0 || r->topk_group > r->n_group) { set_error("moe_router_grouped: topk_group must be 1 .. n_group"); return ZMI_FAILURE; }
