@@ -394,7 +394,8 @@ ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
  * x, A, B: one type, bf16 or f16; dst (and base): bf16, f16 or f32.
  * workspace: device memory of zmi_lora_workspace_size() bytes, 16-byte aligned; null: the calling thread's scratch
  * arena, which a stream that is being captured into a graph cannot use (failure) -- give a captured call a workspace that
- * no other graph shares.  T == 0 is an empty batch: success.
+ * no other graph shares.  T == 0 is an empty batch: success.  The size does not grow with T throughout (fewer rows may be
+ * cut into more parts of K): a workspace for batches of several sizes takes the largest of their sizes.
  * Limits: rank <= 256, n_slices <= ZMI_LORA_MAX_SLICES, n_slots <= 4096, T <= 2^20, K <= 2^19, 2^30 columns. */
 #define ZMI_LORA_MAX_SLICES 4
 typedef struct zmi_lora_t {

@@ -347,3 +347,51 @@ def test_sorted_batches_and_long_runs():
         i32 = dict(dtype=torch.int32, device=H.DEV)
         for ids in ((torch.arange(T, **i32) * 5 // T), torch.zeros(T, **i32), torch.arange(T, **i32).flip(0) * 6 // T - 1):
             Case(T, T, 1024, [264], 32, 5, ids=ids.contiguous()).check("dst")
+
+
+@pytest.mark.parametrize("T", [20, 300])
+@pytest.mark.parametrize("dt,small,large", [(HF, 2.0 ** -24, 2.0 ** 10), (BF, 2.0 ** -131, 2.0 ** 120)])
+def test_subnormal_operands_count(dt, small, large, T):
+    """Subnormal x (and A, and B) against large ones: the products are ordinary values."""
+    g = torch.Generator(device=H.DEV)
+    g.manual_seed(T)
+    whole = lambda *s: torch.randint(-7, 8, s, generator=g, device=H.DEV).double()   # noqa: E731
+    for which in ("x", "a", "b"):
+        c = Case(70, T, 256, [64], 16, 3, dt, F32, mixed=False)
+        c.x = (whole(T, 256) * (small if which == "x" else large if which == "a" else 1.0)).to(dt)
+        c.a = (whole(3, 16, 256) * (small if which == "a" else large if which == "x" else 1.0)).to(dt)
+        c.b = [(whole(3, 64, 16) * (small if which == "b" else 1.0)).to(dt)]
+        if which == "b":
+            c.scales = torch.full((3,), 2.0 ** 20, device=H.DEV)
+        c.check("zero")
+
+
+def test_two_threads_at_once():
+    """Each thread with its own stream (and so its own scratch), small and planned calls in turn."""
+    import threading
+    lib = capi.load()
+    cases = [[Case(80 + k, T, 1024, [320], 32, 4) for T in (24, 700)] for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(mine, s):
+        try:
+            lib.zmi_set_stream(s.cuda_stream)
+            for _ in range(8):
+                for c in mine:
+                    if c.call(c.base) != capi.SUCCESS:
+                        failed.append(lowoha.last_error())
+        finally:
+            lib.zmi_set_stream(None)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for mine in cases:
+        for c in mine:
+            c.compare(c.dst, *c.want(c.base))

@@ -164,10 +164,11 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
 // by global -> LDS loads (DMA), D - 1 stages ahead; otherwise through registers, one stage ahead.
 // The four wavefronts share a stage as WR x WN x WK over row groups, rank tiles and 64-element blocks of K.
 //
-// What bounds it: the cache lines a compute unit can have outstanding (about 90: the sum of all read latencies over the
-// launch's time), 16 clocks a line of x from HBM and 6 a line of A from L2.  206 MB of x and 0.3 GB of A from L2 in the 78 us
-// above, 4.9 TB/s from HBM and L2 together a compute unit's share of 21 bytes a clock; without its arithmetic the launch
-// takes the same time, without its loads 52 us.
+// What bounds it: the cache lines a compute unit can have outstanding.  In the 78 us above 4.3 M lines of 128 bytes (206 MB
+// of x, 346 MB of A read again by every tile; 77 % of the lines come from behind L2) are read with a latency of 806 clocks
+// on average, which is some 70 lines in flight in a compute unit (at 2.4 GHz); without its arithmetic the launch takes the
+// same 78 us, with all loads but the first stages' left out 54.  2048 rows of K = 4096, two slices of rank 32: 13 us for
+// 16 MB of x and A.
 // ---------------------------------------------------------------------------------------------------------------
 template <bool F16, int RT, int NT, int KS, int WR, int WN, int D, bool DMA, bool SMALL>
 __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(ZmiLora p, ZmiLoraPlan w, int ny) {
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
 // ---------------------------------------------------------------------------------------------------------------
 namespace {
 
-// elements of K in a stage of the shrink launch: a stage is 10 .. 24 KiB whatever the tile's shape
+// elements of K in a stage of the shrink launch: a stage is 16 .. 24 KiB whatever the tile's shape
 constexpr int lora_ks(int rt, int nt) { return rt + nt <= 3 ? 256 : rt + nt <= 6 ? 128 : 64; }
 
 int64_t lora_clamp(int64_t v, int64_t lo, int64_t hi) { return v > hi ? (hi < lo ? lo : hi) : v < lo ? lo : v; }
@@ -470,8 +471,8 @@ LoraShape lora_shape(const ZmiLora &p) {
   s.groups = ids + (p.T - ids) / 16;
   const int64_t stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
   // small: K slices of four stages or more (of one where K has few: 301 rows of K = 1001 7.6 us in four slices, 8.6 in one)
-  // while there are less than two workgroups a compute unit (48 rows, 64 slots, three
-  // slices of rank 64 in eights of rank tiles, both launches: 256 workgroups 23.8 us, 512 22.4, 1024 28.5)
+  // while there are less than two workgroups a compute unit (48 rows, 64 slots, three slices of rank 64 in eights of rank
+  // tiles, both launches: 256 workgroups 23.8 us, 512 22.4, 1024 28.5)
   s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages >= 16 ? stages / 4 : stages, 1, 16));
   // planned: a workgroup a compute unit (two share what one already gets through: 512 workgroups 90 us against 82 for 8192
   // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of LORA_RUN stages or more (of two up
@@ -541,8 +542,9 @@ hipError_t launch_shrink(const ZmiLora &p, const ZmiLoraPlan &w, const LoraShape
   constexpr int R2 = RT >= 2 ? 2 : 1;
   if (s.nt == 1) return launch_shrink_as<F16, RT, 1, RT, 1, SMALL>(p, w, s, stream);
   if (s.nt == 2) return launch_shrink_as<F16, RT, 2, RT, RT == 2 ? 2 : 1, SMALL>(p, w, s, stream);
-  if (s.nt == 4) return launch_shrink_as<F16, RT, 4, R2, 4 / R2, SMALL>(p, w, s, stream);
-  return launch_shrink_as<F16, RT, 8, R2, 4 / R2, SMALL>(p, w, s, stream);
+  if constexpr (!SMALL)
+    if (s.nt == 8) return launch_shrink_as<F16, RT, 8, R2, 4 / R2, SMALL>(p, w, s, stream);
+  return launch_shrink_as<F16, RT, 4, R2, 4 / R2, SMALL>(p, w, s, stream);
 }
 
 template <bool F16>

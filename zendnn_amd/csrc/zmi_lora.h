@@ -40,9 +40,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// 16 / 8 bytes at any 2-byte aligned address (global memory takes unaligned vector accesses on this device)
+// 16 bytes at any 2-byte aligned address (global memory takes unaligned vector accesses on this device)
 __device__ __forceinline__ u32x4 load16(const void *p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
-__device__ __forceinline__ void store16(void *p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
 
 // the first n (1 .. 7) of eight 16-bit elements, zeros behind them: four, two and one, as n has them
 __device__ __forceinline__ u32x4 load16_head(const uint16_t *p, int n) {
