@@ -395,3 +395,11 @@ def test_two_threads_at_once():
     for mine in cases:
         for c in mine:
             c.compare(c.dst, *c.want(c.base))
+
+
+@pytest.mark.parametrize("dt,pad", [(BF, 0), (HF, 0), (HF, 5)])
+@pytest.mark.parametrize("T,K,N,rank", [(322, 320, [72], 128), (2100, 328, [64], 128), (4200, 520, [64], 128), (2200, 264, [40], 64),
+                                        (33000, 72, [8], 64), (20000, 264, [16], 32), (33000, 264, [8], 32), (1200, 264, [520, 8], 64)])
+def test_tile_shapes(T, K, N, rank, dt, pad):
+    """Every height of a shrink tile with every number of rank tiles."""
+    Case(T + rank, T, K, N, rank, 2, dt, mixed=False, pad=pad, w_pad=pad).check("other")

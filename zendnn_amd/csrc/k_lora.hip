@@ -467,7 +467,13 @@ LoraShape lora_shape(const ZmiLora &p) {
   const int most = s.small || avg < 20 ? 1 : avg < 48 ? 2 : 4;
   s.rt = s.nt / 2 < 1 ? 1 : s.nt / 2 < most ? s.nt / 2 : most;
   while (s.rt < most && p.T / (32 * s.rt) * s.ny >= 512) s.rt *= 2;
-  s.tiles = ids + (p.T - ids) / (16 * s.rt);
+  const auto tiles_of = [&](int rt) { return ids + (p.T - ids) / (16 * rt); };
+  // Low ones again where there are few: 256 workgroups cut less than 64 units into more than four pieces each, which one
+  // workgroup joins (4 / 2 / 1 groups at rank 128: 322 rows of K = 1120 in one slot 17.3 / 12.1 / 9.6 us, 976 of 10368 in 12
+  // 27.4 / 21.6 / 20.4, 2048 of 4096 in 4 20.3 / 17.2 / 16.6; 2 / 1 at rank 64: 1024 of 4096 in 8 12.8 / 9.3; where there are
+  // 64 it turns: two slices of rank 32, 2048 of 4096 in 4, 12.9 / 15.1).
+  while (s.rt > 1 && tiles_of(s.rt) * s.ny < 64) s.rt /= 2;
+  s.tiles = tiles_of(s.rt);
   s.groups = ids + (p.T - ids) / 16;
   const int64_t stages = (p.K + lora_ks(s.rt, s.nt) - 1) / lora_ks(s.rt, s.nt);
   // small: K slices of four stages or more (of one where K has few: 301 rows of K = 1001 7.6 us in four slices, 8.6 in one)
