@@ -403,3 +403,10 @@ def test_two_threads_at_once():
 def test_tile_shapes(T, K, N, rank, dt, pad):
     """Every height of a shrink tile with every number of rank tiles."""
     Case(T + rank, T, K, N, rank, 2, dt, mixed=False, pad=pad, w_pad=pad).check("other")
+
+
+@pytest.mark.parametrize("rank", [5, 32, 33, 64])
+@pytest.mark.parametrize("dst", [HF, BF])
+def test_f16_columns_of_a_lane(rank, dst):
+    """Eight columns a lane up to rank 32, four beyond: slices that end inside a wavefront's columns, all in eights."""
+    Case(rank, 600, 264, [520, 8, 136], rank, 3, HF, dst).check("dst")

@@ -488,8 +488,11 @@ LoraShape lora_shape(const ZmiLora &p) {
   s.terms = p.dt_dst == ZMI_DT_F32 ? 3 : 2;
   s.dma = p.ldx % 8 == 0 && p.a_ld % 8 == 0 && p.a_slot % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
   s.kt = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : p.rank <= 128 ? 4 : 8;
-  // columns of an expand lane: eight, where the registers hold B of so many and every slice's columns are whole eights
-  bool eights = !s.small && p.dt_x == ZMI_DT_BF16 && p.dt_dst != ZMI_DT_F32 && s.kt < 8;
+  // columns of an expand lane: eight, where the registers hold B of so many and every slice's columns are whole eights (f16,
+  // whose B takes two terms, up to rank 32, four / eight: 2593 rows of 5104 columns at rank 32 25.3 / 19.6 us, 1416 of 9480 at
+  // rank 1 20.8 / 15.9, 1937 of 2792 at rank 24 14.0 / 14.6; with rank 64 eight would gain nothing: 4096 of 4096 22.4 / 22.2,
+  // 600 of 4096 10.7 / 11.9)
+  bool eights = !s.small && p.dt_dst != ZMI_DT_F32 && s.kt <= (p.dt_x == ZMI_DT_BF16 ? 4 : 1);
   for (int i = 0; i < p.n_slices; ++i) eights &= p.N[i] % 8 == 0;
   s.nj = s.kt == 8 ? 2 : eights ? 8 : 4;
   s.col_blocks = 0;

@@ -354,7 +354,7 @@ void launch_as(const ZmiLora &p, const ZmiLoraPlan &w, const LoraShape &s, hipSt
     return;
   }
   const dim3 grid((unsigned)s.col_blocks, (unsigned)s.runs);
-  if constexpr (!F16 && KT < 8 && DST != ZMI_DT_F32) {
+  if constexpr (KT <= (F16 ? 1 : 4) && DST != ZMI_DT_F32) {
     if (s.nj == 8) {
       hipLaunchKernelGGL((zmi_lora_expand_kernel<F16, 8, KT, DST>), grid, block, 0, stream, p, w);
       return;
