@@ -82,6 +82,14 @@ struct Out {
   }
 };
 
+// this lane's number, made where it is used (kept over the whole run of a full wavefront it is a register spilled, and reading
+// it back waits for all loads ahead)
+__device__ __forceinline__ int lane_here() {
+  uint32_t all = ~0u;
+  asm volatile("" : "+s"(all));
+  return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0));
+}
+
 __device__ __forceinline__ u32x4 pack8(const __bf16 (&v)[8]) {
   return __builtin_bit_cast(u32x4, bf16x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]});
 }
@@ -118,7 +126,7 @@ __device__ __forceinline__ void load_b(const ZmiLora &p, int s, int slot, int ra
   for (int c = 0; c < KT; ++c)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      if (F16) {
+      if (F16) {   // (every f16 value is the sum of its two terms)
         float f[8];
         const f16x8 half = __builtin_bit_cast(f16x8, v[c][j]);
 #pragma unroll
@@ -142,6 +150,31 @@ __device__ __forceinline__ void mma_h(f32x4 (&acc)[NJ], u32x4 h, const u32x4 (&b
   if (F16 && !last)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[j] = mma_x<false>(h, b[j][F16 ? 1 : 0], acc[j]);
+}
+
+// An infinite h or B meets zeros and opposite signs among the other operand's terms, which the definition does not know: where
+// the terms' products leave NaN, the sum over the ranks is made again from h and B themselves.  h_of(i, r): h of rank r of
+// row i of the lane's four.
+template <bool F16, int NJ, class H>
+__device__ __forceinline__ void redo_nan(const ZmiLora &p, int s, int slot, int rank, int n, f32x4 (&acc)[NJ], H h_of) {
+  f32x4 top = acc[0];   // (IEEE 754's maximum: NaN where either is)
+#pragma unroll
+  for (int j = 1; j < NJ; ++j) top = __builtin_elementwise_maximum(top, acc[j]);
+  const float any = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top[0], top[1]), __builtin_elementwise_maximum(top[2], top[3]));
+  if (__builtin_expect(any == any, 1)) return;
+  asm volatile("" : "+v"(n));   // (no address of this is made ahead, in registers that the rows in front would lack)
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const uint16_t *b = (const uint16_t *)p.b[s] + slot * p.b_slot[s] + (n + j < p.N[s] ? n + j : p.N[s] - 1) * p.b_ld[s];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // (one at a time: what is live here adds to what the rows in front keep in registers)
+      if (acc[j][i] == acc[j][i]) continue;
+      float sum = 0.0f;
+#pragma unroll 1
+      for (int r = 0; r < rank; ++r) sum = __builtin_fmaf(h_of(i, r), F16 ? zmi_f16_to_f32(b[r]) : zmi_bf16_to_f32(b[r]), sum);
+      acc[j][i] = sum;
+    }
+  }
 }
 
 }  // namespace
@@ -197,17 +230,18 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
     u32x4 b[KT][NJ][F16 ? 2 : 1];
     typename O::run_t y[4], y_next[4], out[4];
     int4 rows = rows_of(a), rows_next = rows_of(a + 1 < z ? a + 1 : a), rows_out = rows;
-    int slot = -1, kts = 0;
+    int slot = -1, rank = 0, kts = 0;
     float scale = 0.0f;
     auto take_slot = [&](int i) {
       const int now = __builtin_amdgcn_readfirstlane(w.group_slot[2 * i]);
       if (now == slot) return;
       slot = now;
-      const int rank = __builtin_amdgcn_readfirstlane(w.group_slot[2 * i + 1]);
+      rank = __builtin_amdgcn_readfirstlane(w.group_slot[2 * i + 1]);
       kts = (rank + 31) / 32;
       if (!kts) return;
       scale = p.scales ? p.scales[slot] : 1.0f;
       load_b<F16, NJ, KT>(p, s, slot, rank, n, b);
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // (waited for here, B holds up no group of the same slot until the loads ahead are back)
     };
     send_h(a);
     if (here) {
@@ -226,6 +260,7 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
         if (i > a) store(out, rows_out);
         take_slot(i);
         if (kts) {
+          const char *const h_at = ring[i & 1] + lane_here() * 16;
           f32x4 acc[NJ];
 #pragma unroll
           for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
@@ -233,8 +268,15 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
           for (int c = 0; c < KT; ++c) {
             if (c >= kts) break;
 #pragma unroll
-            for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, *(const u32x4 *)(ring[i & 1] + (c * TERMS + k) * 1024 + lane * 16), b[c], k + 1 == TERMS);
+            for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, *(const u32x4 *)(h_at + (c * TERMS + k) * 1024), b[c], k + 1 == TERMS);
           }
+          redo_nan<F16, NJ>(p, s, slot, rank, n, acc, [&](int q, int r) {
+            const char *at = ring[i & 1] + r / 32 * TERMS * 1024 + (r / 8 % 4 * 16 + g * 4 + q) * 16 + r % 8 * 2;
+            float h = 0.0f;
+#pragma unroll
+            for (int k = TERMS - 1; k >= 0; --k) h += zmi_bf16_to_f32(*(const uint16_t *)(at + k * 1024));
+            return h;
+          });
 #pragma unroll
           for (int r = 0; r < 4; ++r) out[r] = O::sum(y[r], acc, r, scale);
         } else {
@@ -330,6 +372,13 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_small_kern
 #pragma unroll
         for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, pack8(h[k]), b[c], k + 1 == TERMS);
       }
+      redo_nan<F16, NJ>(p, s, slot, rank, n, acc, [&](int i, int r) {
+        if (g * 4 + i >= count) return 0.0f;
+        const float *src = w.partial + (((int64_t)blockIdx.y * qt + s * lt + r / 16) * 64 + r % 16 / 4 * 16 + g * 4 + i) * 4 + r % 4;
+        float h = 0.0f;
+        for (int k = 0; k < slices; ++k) h += src[(int64_t)k * gridDim.y * qt * 256];
+        return h;
+      });
       if (kts) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = O::sum(y[i], acc, i, scale);

@@ -196,17 +196,19 @@ __device__ __forceinline__ f32x4 mma_x(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// v as TERMS bf16 terms, largest first; what is left of a value that is not finite is zero
+// v as TERMS bf16 terms, largest first.  A finite value's terms are finite (bf16's largest stands for what would round beyond
+// it, the next term holds the rest); what is left of a value that is not finite is zero.
 template <int TERMS, int N>
 __device__ __forceinline__ void split(const float (&v)[N], __bf16 (&t)[TERMS][N]) {
+  const float most = 0x1.fep127f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float rest = v[i];
+    const bool finite = __builtin_fabsf(rest) < __builtin_inff();
 #pragma unroll
     for (int k = 0; k < TERMS; ++k) {
-      t[k][i] = (__bf16)rest;
-      const float hi = (float)t[k][i];
-      rest = __builtin_fabsf(hi) < __builtin_inff() ? rest - hi : 0.0f;
+      t[k][i] = (__bf16)(k == 0 && finite ? __builtin_amdgcn_fmed3f(rest, -most, most) : rest);
+      rest = finite ? rest - (float)t[k][i] : 0.0f;
     }
   }
 }
