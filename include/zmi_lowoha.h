@@ -386,11 +386,12 @@ ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
  * gate / up projection has several; slice s covers N[s] columns behind those of the slices before it):
  *   h[r]      = sum_k x[t][k] * A[a][s * rank + r][k],                            r < ranks[a]
  *   dst[t][n] = base[t][n] + scales[a] * sum_r h[r] * B_s[a][n][r]
- * Sums are f32, h keeps at least 16 bits of its values' precision in front of the second product, and dst is rounded
- * once, to nearest even.  An infinity or NaN in x, A or B reaches what these sums take it to, and nothing else.  base may be dst itself (same pointer and stride: the rows of dst get their adapters' part
- * added, rows without an adapter are left as they are), another buffer of dst's type, or null (zero).  A slot id outside
- * [0, n_slots) means no adapter: dst = base.  ranks (null: `rank` for all) holds the rank of the adapter in each slot,
- * taken as 0 .. rank; what the slot holds beyond it is not used.  scales null: 1.
+ * Sums are f32, h goes into the second product with all bits that f32 holds (down to 2^-133), and dst is rounded once, to
+ * nearest even.  An infinity or NaN in x, A or B reaches what these sums take it to, and nothing else.
+ * base may be dst itself (same pointer and stride: the rows of dst get their adapters' part added, rows without an adapter
+ * are left as they are), another buffer of dst's type, or null (zero).  A slot id outside [0, n_slots) means no adapter:
+ * dst = base.  ranks (null: `rank` for all) holds the rank of the adapter in each slot, taken as 0 .. rank; what the slot
+ * holds beyond it is not used.  scales null: 1.
  * x, A, B: one type, bf16 or f16; dst (and base): bf16, f16 or f32.
  * workspace: device memory of zmi_lora_workspace_size() bytes, 16-byte aligned; null: the calling thread's scratch
  * arena, which a stream that is being captured into a graph cannot use (failure) -- give a captured call a workspace that

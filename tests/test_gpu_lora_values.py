@@ -1,4 +1,4 @@
-"""GPU tests of the values of zmi_lora_direct: infinite and huge operands."""
+"""GPU tests of the values of zmi_lora_direct: infinite and huge operands, and the precision that h is held in."""
 import pytest
 import torch
 
@@ -100,3 +100,26 @@ def test_h_between_the_largest_bf16_and_the_largest_f32(T, dst):
     assert c.call(None) == capi.SUCCESS, lowoha.last_error()
     want = (sign.double() * (2 - 2.0 ** -9) * 2.0 ** 27).to(dst)[:, None].expand(-1, 40)
     assert torch.equal(c.dst, want)
+
+@pytest.mark.parametrize("T", [1, 40, 300, 700])
+@pytest.mark.parametrize("dt,dst", [(BF, BF), (BF, HF), (BF, F32), (HF, HF), (HF, BF), (HF, F32)])
+def test_h_keeps_24_bits(T, dt, dst):
+    """h of 22 bits, exact in f32, next to a base that cancels all but its lowest ones: what is left is exact, and dst is its
+    rounding."""
+    c = Case(T, T, 64, [40], 8, 2, dt, dst, mixed=False, none=0.0, scales=False)
+    g = torch.Generator(device=H.DEV)
+    g.manual_seed(T)
+    c.x.zero_()
+    c.x[:, 0], c.x[:, 1], c.x[:, 2] = 1.0, 2.0 ** -8, 2.0 ** -15
+    a = 1.0 + torch.randint(0, 128, (2, 8, 64), generator=g, device=H.DEV) / 128.0   # 8 bits: h has 1 + 22 of them
+    c.a.copy_(a)
+    c.b[0].zero_()
+    rank_of = torch.randint(0, 8, (2, 40), generator=g, device=H.DEV)
+    c.b[0].scatter_(2, rank_of[:, :, None], 1.0)
+    h = c.x[:, :3].double()[:, None, :] * c.a.double()[c.ids.long()][:, :, :3]
+    h = torch.gather(h.sum(2), 1, rank_of[c.ids.long()])
+    assert torch.equal(h, h.float().double())
+    c.base.copy_(-h)                                 # (rounded to dst's type)
+    want = (h + c.base.double()).to(dst)
+    assert c.call(c.base) == capi.SUCCESS, lowoha.last_error()
+    assert torch.equal(c.dst, want), float((c.dst.double() - want.double()).abs().max())

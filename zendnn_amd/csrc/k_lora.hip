@@ -11,11 +11,9 @@
 //   shrink  h of a tile, K through an LDS ring.  K is cut into slices where the tiles alone do not fill the device;
 //   expand  dst.  A wavefront keeps 32 .. 128 columns' B in registers and goes down the rows of its slot.
 //
-// The MFMA takes 16-bit operands: x, A exactly as they are; h, which is f32, as a sum of bf16 terms (2 terms hold 16
-// bits, for f32 destinations 3 hold 24), and f16 B, which the range of h does not allow to meet in f16, as two bf16 terms
-// that hold it exactly.  All products are accumulated in f32.
-#include <type_traits>
-
+// The MFMA takes 16-bit operands: x, A exactly as they are; h, which is f32, as a sum of three bf16 terms, which hold all of
+// its 24 bits (down to bf16's least value, 2^-133), and f16 B, which the range of h does not allow to meet in f16, as two bf16
+// terms that hold it exactly.  All products are accumulated in f32.
 #include "zmi_lora.h"
 
 #define LORA_RUN 4   // least stages of a shrink workgroup's run
@@ -338,21 +336,16 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_shrink_kernel(Zmi
       float f[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = r + e < rank ? v[e] : 0.0f;
-      auto put = [&](auto terms) {
-        constexpr int TERMS = decltype(terms)::value;
-        __bf16 h[TERMS][4];
-        split<TERMS>(f, h);
-        char *to = (char *)w.h + ((((int64_t)(t.group + i) * p.n_slices + s) * kt + r / 32) * TERMS) * 1024 +
-                   (r / 8 % 4 * 16 + c16) * 16 + r % 8 * 2;
+      __bf16 h[LORA_TERMS][4];
+      split<LORA_TERMS>(f, h);
+      char *to = (char *)w.h + ((((int64_t)(t.group + i) * p.n_slices + s) * kt + r / 32) * LORA_TERMS) * 1024 +
+                 (r / 8 % 4 * 16 + c16) * 16 + r % 8 * 2;
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          *(bf16x4 *)(to + k * 1024) = bf16x4{h[k][0], h[k][1], h[k][2], h[k][3]};
-          // (a block whose upper half no rank tile fills)
-          if (q - s * lt == lt - 1 && lt % 2) *(u32x2 *)(to + k * 1024 + 512) = u32x2{0, 0};
-        }
-      };
-      if (p.dt_dst == ZMI_DT_F32) put(std::integral_constant<int, 3>());
-      else put(std::integral_constant<int, 2>());
+      for (int k = 0; k < LORA_TERMS; ++k) {
+        *(bf16x4 *)(to + k * 1024) = bf16x4{h[k][0], h[k][1], h[k][2], h[k][3]};
+        // (a block whose upper half no rank tile fills)
+        if (q - s * lt == lt - 1 && lt % 2) *(u32x2 *)(to + k * 1024 + 512) = u32x2{0, 0};
+      }
     };
     // where a piece's sums stand: small [K slice][tile][rank tile][lane], planned a workgroup's first and last piece
     auto small_at = [&](int q) { return w.partial + ((((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * qt + q) * 64 + lane) * 4; };
@@ -485,7 +478,6 @@ LoraShape lora_shape(const ZmiLora &p) {
   // to 128 workgroups)
   const int64_t all = s.tiles * s.ny * stages, few = lora_clamp(all / 2, 8, 128);
   s.grid = (int)lora_clamp(all / LORA_RUN, few, 256) / 8 * 8;
-  s.terms = p.dt_dst == ZMI_DT_F32 ? 3 : 2;
   s.dma = p.ldx % 8 == 0 && p.a_ld % 8 == 0 && p.a_slot % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
   s.kt = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : p.rank <= 128 ? 4 : 8;
   // columns of an expand lane: eight, where the registers hold B of so many and every slice's columns are whole eights (f16,
@@ -519,7 +511,7 @@ size_t lora_layout(const ZmiLora &p, const LoraShape &s, char *base, ZmiLoraPlan
     l.place = (int32_t *)take(p.T > LORA_PLAN_KEEP * 256 ? (size_t)p.T * 4 : 0);
     l.n_arrivals = (int32_t)(s.tiles * s.ny);
     l.arrivals = (uint32_t *)take((size_t)l.n_arrivals * 4);
-    l.h = take((size_t)s.groups * p.n_slices * ((p.rank + 31) / 32) * s.terms * 1024);
+    l.h = take((size_t)s.groups * p.n_slices * ((p.rank + 31) / 32) * LORA_TERMS * 1024);
     l.partial = (float *)take((size_t)s.grid * 2 * s.rt * s.nt * 1024);
   } else {
     l.tiles = (int32_t *)take((size_t)s.tiles * 80);

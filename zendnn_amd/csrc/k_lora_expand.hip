@@ -18,7 +18,6 @@ namespace {
 template <int NJ, int DST>   // DST: ZMI_DT_*
 struct Out {
   static constexpr int ES = DST == ZMI_DT_F32 ? 4 : 2, BYTES = NJ * ES, WORDS = BYTES / 4;
-  static constexpr int TERMS = DST == ZMI_DT_F32 ? 3 : 2;
   static constexpr int COLS = LORA_WAVES * 16 * NJ;   // of a workgroup
   typedef uint32_t run_t __attribute__((ext_vector_type(WORDS)));   // a lane's columns of a row
 
@@ -141,12 +140,12 @@ __device__ __forceinline__ void load_b(const ZmiLora &p, int s, int slot, int ra
     }
 }
 
-// acc += h (term k of `terms`) times B
+// acc += a term of h times B
 template <bool F16, int NJ>
 __device__ __forceinline__ void mma_h(f32x4 (&acc)[NJ], u32x4 h, const u32x4 (&b)[NJ][F16 ? 2 : 1], bool last) {
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = mma_x<false>(h, b[j][0], acc[j]);
-  // (the product of the last terms is beyond the precision kept)
+  // (the last terms' product is at most 2^-25 of the whole one, less than a rounding of the sum)
   if (F16 && !last)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[j] = mma_x<false>(h, b[j][F16 ? 1 : 0], acc[j]);
@@ -183,8 +182,7 @@ __device__ __forceinline__ void redo_nan(const ZmiLora &p, int s, int slot, int 
 template <bool F16, int NJ, int KT, int DST>
 __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(ZmiLora p, ZmiLoraPlan w) {
   typedef Out<NJ, DST> O;
-  constexpr int TERMS = O::TERMS;
-  __shared__ __attribute__((aligned(16))) char ring[2][KT * TERMS * 1024];
+  __shared__ __attribute__((aligned(16))) char ring[2][KT * LORA_TERMS * 1024];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = lane / 16, c16 = lane % 16;
   // (in place the rows without an adapter, which come last, are left alone)
   const int64_t groups = __builtin_amdgcn_readfirstlane(w.header[p.base == p.dst ? 1 : 2]);
@@ -201,9 +199,9 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
 
   auto rows_of = [&](int i) { return *(const int4 *)(w.order + (int64_t)i * 16 + g * 4); };
   auto send_h = [&](int i) {   // 1 KiB operand blocks, as many as the group's adapter has
-    const int units = (w.group_slot[2 * i + 1] + 31) / 32 * TERMS;
+    const int units = (w.group_slot[2 * i + 1] + 31) / 32 * LORA_TERMS;
     const uint32_t into = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)(char *)ring[i & 1]);
-    const char *from = (const char *)w.h + ((int64_t)i * p.n_slices + s) * kt * TERMS * 1024 + lane * 16;
+    const char *from = (const char *)w.h + ((int64_t)i * p.n_slices + s) * kt * LORA_TERMS * 1024 + lane * 16;
     for (int u = wave; u < units; u += LORA_WAVES)
       asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
                    ::"s"(into + u * 1024), "v"(from + u * 1024) : "memory", "m0");
@@ -268,13 +266,13 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
           for (int c = 0; c < KT; ++c) {
             if (c >= kts) break;
 #pragma unroll
-            for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, *(const u32x4 *)(h_at + (c * TERMS + k) * 1024), b[c], k + 1 == TERMS);
+            for (int k = 0; k < LORA_TERMS; ++k) mma_h<F16, NJ>(acc, *(const u32x4 *)(h_at + (c * LORA_TERMS + k) * 1024), b[c], k + 1 == LORA_TERMS);
           }
           redo_nan<F16, NJ>(p, s, slot, rank, n, acc, [&](int q, int r) {
-            const char *at = ring[i & 1] + r / 32 * TERMS * 1024 + (r / 8 % 4 * 16 + g * 4 + q) * 16 + r % 8 * 2;
+            const char *at = ring[i & 1] + r / 32 * LORA_TERMS * 1024 + (r / 8 % 4 * 16 + g * 4 + q) * 16 + r % 8 * 2;
             float h = 0.0f;
 #pragma unroll
-            for (int k = TERMS - 1; k >= 0; --k) h += zmi_bf16_to_f32(*(const uint16_t *)(at + k * 1024));
+            for (int k = LORA_TERMS - 1; k >= 0; --k) h += zmi_bf16_to_f32(*(const uint16_t *)(at + k * 1024));
             return h;
           });
 #pragma unroll
@@ -302,7 +300,6 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
 template <bool F16, int NJ, int KT, int DST>
 __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_small_kernel(ZmiLora p, ZmiLoraPlan w, int slices) {
   typedef Out<NJ, DST> O;
-  constexpr int TERMS = O::TERMS;
   const int lane = threadIdx.x % 64, g = lane / 16, c16 = lane % 16;
   // the tile as the shrink launch found it
   const int32_t *entry = w.tiles + blockIdx.y * 20;
@@ -367,10 +364,10 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_small_kern
           for (int e = 0; e < 8; ++e)
             if (e >= left) v[e] = 0.0f;
         }
-        __bf16 h[TERMS][8];
-        split<TERMS>(v, h);
+        __bf16 h[LORA_TERMS][8];
+        split<LORA_TERMS>(v, h);
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k) mma_h<F16, NJ>(acc, pack8(h[k]), b[c], k + 1 == TERMS);
+        for (int k = 0; k < LORA_TERMS; ++k) mma_h<F16, NJ>(acc, pack8(h[k]), b[c], k + 1 == LORA_TERMS);
       }
       redo_nan<F16, NJ>(p, s, slot, rank, n, acc, [&](int i, int r) {
         if (g * 4 + i >= count) return 0.0f;

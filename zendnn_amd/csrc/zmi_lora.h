@@ -4,6 +4,7 @@
 #include "zmi_launch.h"
 
 #define LORA_WAVES 4
+#define LORA_TERMS 3   // bf16 terms that h is held in: 24 bits, all that f32 has
 // Rows up to which wavefronts plan for themselves: any slots, or few slots and ranks (a round of the search per distinct slot,
 // and a tile's 16 rows read all of their slot's A and B)
 #define LORA_SMALL_T 128
@@ -26,7 +27,6 @@ struct LoraShape {
   int nj;              // its column tiles of 16
   int64_t col_blocks;
   int64_t runs;        // planned: expand workgroups down the rows
-  int terms;
 };
 
 hipError_t lora_launch_expand(const ZmiLora &p, const ZmiLoraPlan &w, const LoraShape &s, hipStream_t stream);
