@@ -73,6 +73,17 @@ __device__ __forceinline__ float rgk_exp_down(float d) {
   return __builtin_fmaf(e, r * 0.693147182464599609375f, e);
 }
 
+// exp(d) in 64 bits, to 2^-31.7 of its value: exp(n ln 2) exp(r) with |r| <= ln 2 / 2, whose series ends at r^8 / 8!  (what the
+// weights need and no more: 64 x 64 logits 3.33 us, with the library's exp 3.45)
+__device__ __forceinline__ double rgk_exp64(double d) {
+  d = d < -1100.0 ? -1100.0 : d > 1100.0 ? 1100.0 : d;   // (beyond are 0 and infinity; NaN stays)
+  const double n = __builtin_rint(d * 1.4426950408889634), r = __builtin_fma(n, -0.6931471805599453, d), r2 = r * r;
+  const double low = __builtin_fma(__builtin_fma(r, 1.0 / 6, 0.5), r2, 1.0 + r);
+  const double high = __builtin_fma(__builtin_fma(r, 1.0 / 5040, 1.0 / 720), r2, __builtin_fma(r, 1.0 / 120, 1.0 / 24));
+  const double r4 = r2 * r2;
+  return __builtin_ldexp(__builtin_fma(__builtin_fma(r4, 1.0 / 40320, high), r4, low), (int)n);
+}
+
 // value -> unsigned key in the values' order; -0 == +0; NaN 1, below every number (0: nothing)
 __device__ __forceinline__ uint32_t rgk_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
@@ -317,13 +328,11 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
     }
     rgk_choose<J>(p, key64, v64, 0.0f, scratch[wave], &mine);
   }
-  // ---- weights: exponentials in f32, the rest in 64 bits ----
+  // ---- weights, in 64 bits: y - m rounded to f32 would be off by more the further an expert lies below the best ----
   double s = 0.0;
   if (lane < p.topk) {
-    const float y = zmi_ld_f32(p.logits, p.logits_dt, row + mine), d = SIGMOID ? -y : y - m;
-    double e = (double)zmi_expf(d);
-    // (scores near the end of f32's range count where all chosen are there)
-    if (__builtin_fabsf(d) >= 80.0f) e = exp(SIGMOID ? -(double)y : (double)y - (double)m);
+    const float y = zmi_ld_f32(p.logits, p.logits_dt, row + mine);
+    const double e = rgk_exp64(SIGMOID ? -(double)y : (double)y - (double)m);
     s = SIGMOID ? 1.0 / (1.0 + e) : y == -__builtin_inff() ? 0.0 : y == m ? 1.0 : e;
   }
   const double z = p.renormalize ? rgk_wave_sum(s) : SIGMOID ? 1.0 : sum;
