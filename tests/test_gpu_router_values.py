@@ -50,3 +50,38 @@ def test_weights_where_the_roundings_of_x_minus_m_add_up(E):
     x[:, 3] += np.float32(u)
     check(H.to_dev(x), min(E, 64), capi.SCORE_SOFTMAX)
     check(H.to_dev(-x), min(E, 64), capi.SCORE_SOFTMAX)
+
+
+@pytest.mark.parametrize("scoring", [capi.SCORE_SOFTMAX, capi.SCORE_SIGMOID])
+@pytest.mark.parametrize("E", [512, 500, 300])
+@pytest.mark.parametrize("topk", [4, 8, 10, 12, 16, 32, 64])
+@pytest.mark.parametrize("together", [2, 3, 4, 5, 8, 11])
+def test_best_experts_next_to_each_other(scoring, E, topk, together):
+    """More than 256 experts stand in eights: tokens whose best ones share an eight, at its start and across its end."""
+    rng = np.random.default_rng(E + topk + together)
+    x = rng.standard_normal((48, E)).astype(np.float32)
+    bias = (rng.standard_normal(E) * 0.01).astype(np.float32)
+    for t in range(48):
+        at = min((t * 8 + (0 if t % 3 else 3)) % E, E - together)
+        x[t, at:at + together] += np.float32(4.0)
+        if t % 4 == 0:      # two such places, one of them at the border of the choice
+            at = (at + E // 2) % (E - together)
+            x[t, at:at + together] = np.sort(x[t])[-topk] + rng.permutation(together).astype(np.float32) * np.float32(1e-2)
+        if t % 5 == 0:      # equal ones
+            x[t, at:at + together] = x[t, at]
+    for b in (None, bias, np.zeros(E, dtype=np.float32)):
+        check(H.to_dev(x), topk, scoring, b, renormalize=True)
+
+
+@pytest.mark.parametrize("E,n_group,topk_group,topk", [(512, 8, 1, 8), (512, 8, 1, 64), (512, 64, 2, 16), (512, 64, 1, 8), (320, 64, 1, 5),
+                                                       (320, 64, 3, 12), (500, 50, 2, 20), (300, 4, 1, 40), (512, 8, 2, 4), (512, 8, 2, 33)])
+@pytest.mark.parametrize("scoring", [capi.SCORE_SOFTMAX, capi.SCORE_SIGMOID])
+@pytest.mark.parametrize("biased", [False, True])
+def test_many_of_the_experts_of_few_groups(E, n_group, topk_group, topk, scoring, biased):
+    rng = np.random.default_rng(E + topk)
+    x = rng.standard_normal((64, E)).astype(np.float32)
+    bias = (rng.standard_normal(E) * 0.05).astype(np.float32) if biased else None
+    check(H.to_dev(x), topk, scoring, bias, n_group, topk_group, False, True)
+    check(H.to_dev(x), topk, scoring, bias, n_group, topk_group, True, False)
+    x = np.round(x * 4) / 4          # many equal values
+    check(H.to_dev(x.astype(np.float32)), topk, scoring, bias, n_group, topk_group, True, True)

@@ -96,8 +96,9 @@ __device__ __forceinline__ uint64_t rgk_key(double x) {
 __device__ __forceinline__ float rgk_value(uint32_t k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ double rgk_value(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k)); }
 
-// The DEPTH largest of a lane's J keys in descending order, equal ones in ascending j (neighbours are exchanged only when out
-// of order); returns the j of each, four bits apiece, the first in the lowest bits, and ones behind them.
+// The DEPTH largest of a lane's J keys in descending order in front of the others, equal ones in ascending j (neighbours are
+// exchanged only when out of order); returns the j of each, four bits apiece, the first in the lowest bits, and ones behind
+// them.
 template <int J, int DEPTH, class K>
 __device__ __forceinline__ uint32_t rgk_sort(K (&key)[J]) {
   // (a vector, not an array: choosing between two elements of an array becomes an indexed read, a chain of comparisons)
@@ -128,14 +129,55 @@ __device__ __forceinline__ void rgk_pair(K &a, K &b) {
   a = max(a, c);
 }
 
+// The rounds of the choice, on V's keys: the largest first key of a lane, of the lowest lane that has it.  A lane gives up to
+// DEPTH of its J; false where the one behind them might have been chosen, or where a gap that decides is not wide enough.
+template <int J, int DEPTH, class V, class K>
+__device__ __forceinline__ bool rgk_rounds(const ZmiRouterGrouped &p, K (&key)[J], float score, int *mine) {
+  const int lane = threadIdx.x % 64;
+  uint32_t queue = rgk_sort<J, DEPTH>(key);
+  uint32_t order = 0;   // float values: lane r keeps the r-th key
+  for (int r = 0; r < p.topk; ++r) {
+    const K top = rgk_wave_max(key[0]);
+    const int at = __builtin_ctzll(__ballot(key[0] == top));
+    const int e = at * J + (__builtin_amdgcn_readlane((int)queue, at) & 15);
+    if (lane == r) { *mine = e; order = (uint32_t)top; }
+    if (lane == at) {
+#pragma unroll
+      for (int j = 0; j + 1 < DEPTH; ++j) key[j] = key[j + 1];
+      key[DEPTH - 1] = 0;
+      queue = DEPTH < 8 ? (uint32_t)((int32_t)queue >> 4) : queue >> 4;
+    }
+  }
+  if (DEPTH < J) {
+    const bool empty = (queue & 15) == 15;
+    if (__ballot(empty)) {
+      K hidden = 0;
+#pragma unroll
+      for (int j = DEPTH; j < J; ++j) hidden = max(hidden, key[j]);
+      if (empty) key[0] = hidden;
+      if (__ballot(empty && hidden >= (K)(uint32_t)__builtin_amdgcn_readlane((int)order, p.topk - 1))) return false;
+    }
+  }
+  if (std::is_same<V, float>::value && p.bias) {
+    const uint32_t rest = (uint32_t)rgk_wave_max(key[0]), below = (uint32_t)__shfl_down((int)order, 1, 64);
+    const uint32_t next = lane == p.topk - 1 ? rest : below;
+    const float a = rgk_value(order), b = rgk_value(next);
+    const bool close = lane < p.topk && next && !(a - b > 0x1p-19f * score + 0x1p-23f * (__builtin_fabsf(a) + __builtin_fabsf(b)));
+    if (__ballot(close)) return false;
+  }
+  return true;
+}
+
 // The choice.  key: what experts are ordered by, v: the values that groups are valued by (top2); both of V's type.  Lane r
 // gets the r-th expert.
 //
-// Float keys (with a bias) and v are f32 values of scores up to `score`: false when a gap that decides is not wide enough.
-// A score is at most 4 ulp off, 2^-21 score, and rounding a value adds half an ulp of it, so two values that lie
-// 2^-20 score + 2^-24 (|a| + |b|) apart are in the order of the exact ones; twice that is asked for.  Values below the one
-// compared with can be off by more where they are larger, but then they are negative and far below.
-template <int J, class V, class K>
+// Float keys (with a bias) and v are f32 values of scores up to `score`: false when a gap that decides is not wide enough.  What
+// the f32 scores of two experts are off by, in half steps of 2^-24 `score`, all of them the other way: sigmoids 7 each
+// (exponential 4, addition 1, reciprocal 2); softmax scores 5.4 each (exponential 4, product 1, x - m in front of it 0.4 at the
+// most) and 13 of their difference (the sum, and its inverse), 19 together.  32 are asked for, and for two groups of two
+// experts 64, where at most 38 meet; rounding a value adds half an ulp of it, which is asked for twice.
+// Values below the one compared with can be off by more where they are larger, but then they are negative and far below.
+template <int J, int SORT, class V, class K>
 __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J], const V (&v)[J], float score, void *scratch, int *mine) {
   const int lane = threadIdx.x % 64, e0 = lane * J, n = p.E - e0, per = p.per;
   if (p.topk_group < p.n_group) {
@@ -192,37 +234,12 @@ __device__ __forceinline__ bool rgk_choose(const ZmiRouterGrouped &p, K (&key)[J
       if (j < n && !((groups >> of) & 1u)) key[j] = 0;
     }
   }
-  // rounds: the largest first key of a lane, of the lowest lane that has it.  Of eight experts a lane sorts three: that a lane
-  // has to give more happens to one token in some thousands, which is then chosen again from whole lanes.
-  constexpr int DEPTH = std::is_same<V, float>::value && J > 4 ? 3 : J;
-  uint32_t queue = rgk_sort<J, DEPTH>(key);
-  uint32_t order = 0;   // float values: lane r keeps the r-th key
-  for (int r = 0; r < p.topk; ++r) {
-    const K top = rgk_wave_max(key[0]);
-    const int at = __builtin_ctzll(__ballot(key[0] == top));
-    const int e = at * J + (__builtin_amdgcn_readlane((int)queue, at) & 15);
-    if (lane == r) { *mine = e; order = (uint32_t)top; }
-    if (lane == at) {
-#pragma unroll
-      for (int j = 0; j + 1 < DEPTH; ++j) key[j] = key[j + 1];
-      key[DEPTH - 1] = 0;
-      queue = DEPTH < 8 ? (uint32_t)((int32_t)queue >> 4) : queue >> 4;
-    }
-  }
-  if (DEPTH < J && __ballot((queue & 15) == 15)) return false;
-  if (std::is_same<V, float>::value && p.bias) {
-    const uint32_t rest = (uint32_t)rgk_wave_max(key[0]), below = (uint32_t)__shfl_down((int)order, 1, 64);
-    const uint32_t next = lane == p.topk - 1 ? rest : below;
-    const float a = rgk_value(order), b = rgk_value(next);
-    const bool close = lane < p.topk && next && !(a - b > 0x1p-19f * score + 0x1p-23f * (__builtin_fabsf(a) + __builtin_fabsf(b)));
-    if (__ballot(close)) return false;
-  }
-  return true;
+  return rgk_rounds<J, std::is_same<V, float>::value ? SORT : J, V>(p, key, score, mine);
 }
 
 }  // namespace
 
-template <int J, bool SIGMOID>
+template <int J, bool SIGMOID, int SORT>   // SORT: experts that a lane sorts for the choice on f32 values
 __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(ZmiRouterGrouped p) {
   __shared__ double scratch[RGK_WAVES][64 * J];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -309,7 +326,7 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
     for (int j = 0; j < J; ++j) key[j] = j < n ? rgk_key(x[j]) : 0u;
   }
   int mine = 0;
-  if (!rgk_choose<J>(p, key, v, score, scratch[wave], &mine)) {
+  if (!rgk_choose<J, SORT>(p, key, v, score, scratch[wave], &mine)) {
     double v64[J];
     uint64_t key64[J];
     double z = 0.0;
@@ -326,7 +343,7 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
       v64[j] += (double)bias[j];
       key64[j] = j >= n ? 0u : p.bias ? rgk_key(v64[j]) : rgk_key((double)x[j]);
     }
-    rgk_choose<J>(p, key64, v64, 0.0f, scratch[wave], &mine);
+    rgk_choose<J, SORT>(p, key64, v64, 0.0f, scratch[wave], &mine);
   }
   // ---- weights, in 64 bits: y - m rounded to f32 would be off by more the further an expert lies below the best ----
   double s = 0.0;
@@ -344,11 +361,11 @@ __global__ __launch_bounds__(RGK_WAVES * 64) void zmi_moe_router_grouped_kernel(
 
 namespace {
 
-template <int J>
+template <int J, int SORT = J>
 void rgk_launch(const ZmiRouterGrouped &p, hipStream_t stream) {
   const dim3 grid((unsigned)((p.T + RGK_WAVES - 1) / RGK_WAVES)), block(RGK_WAVES * 64);
-  if (p.sigmoid) hipLaunchKernelGGL((zmi_moe_router_grouped_kernel<J, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((zmi_moe_router_grouped_kernel<J, false>), grid, block, 0, stream, p);
+  if (p.sigmoid) hipLaunchKernelGGL((zmi_moe_router_grouped_kernel<J, true, SORT>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((zmi_moe_router_grouped_kernel<J, false, SORT>), grid, block, 0, stream, p);
 }
 
 }  // namespace
@@ -363,9 +380,16 @@ hipError_t zmi_launch_moe_router_grouped(ZmiRouterGrouped p, hipStream_t stream)
   p.per = p.E / p.n_group;
   p.inv_per = 1.0f / (float)p.per;   // (e + 0.5) times it truncates to e / per for every e < 512
   p.lane_shift = p.per % J == 0 && lanes <= 16 && (lanes & (lanes - 1)) == 0 ? __builtin_ctz(lanes) : -1;
+  // Of eight experts a lane sorts three, unless too many tokens would have four of their best in one lane, be short of the fourth
+  // and chosen again: topk^4 / 24 sets of four, each in one of the live lanes with 1 / lanes^3; at more than one token in 128
+  // a lane sorts all eight, with a bias, where that costs more, at one in 16 (16384 x 512 softmax, three / eight: topk 10
+  // 20.7 / 21.7 us, 16 25.8 / 25.2, 32 44.3 / 35.8, 64 116.7 / 56.3; with a bias 16 25.9 / 29.2, 32 41.0 / 44.3, 64 107 / 74; 8
+  // experts of one group of 64 29.5 / 25.9, of two 25.6 / 26.8, 12 of two 32.6 / 30.4).
+  const int64_t live = p.topk_group * p.per / 8 + 1, sets = (int64_t)p.topk * (p.topk - 1) * (p.topk - 2) * (p.topk - 3) / 24;
   if (J == 1) rgk_launch<1>(p, stream);
   else if (J == 2) rgk_launch<2>(p, stream);
   else if (J == 4) rgk_launch<4>(p, stream);
-  else rgk_launch<8>(p, stream);
+  else if (sets * (p.bias ? 16 : 128) > live * live * live) rgk_launch<8>(p, stream);
+  else rgk_launch<8, 3>(p, stream);
   return hipGetLastError();
 }
