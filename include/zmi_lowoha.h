@@ -389,7 +389,8 @@ ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
  * Sums are f32, h goes into the second product with all bits that f32 holds (down to 2^-133), and dst is rounded once, to
  * nearest even.  An infinity or NaN in x, A or B reaches what these sums take it to, and nothing else.
  * base may be dst itself (same pointer and stride: the rows of dst get their adapters' part added, rows without an adapter
- * are left as they are), another buffer of dst's type, or null (zero).  A slot id outside [0, n_slots) means no adapter:
+ * are left as they are), rows of dst's type that share no byte with dst's (failure if they do; columns of one buffer beside
+ * each other are fine), or null (zero); dst overlaps no other operand.  A slot id outside [0, n_slots) means no adapter:
  * dst = base.  ranks (null: `rank` for all) holds the rank of the adapter in each slot, taken as 0 .. rank; what the slot
  * holds beyond it is not used.  scales null: 1.
  * x, A, B: one type, bf16 or f16; dst (and base): bf16, f16 or f32.

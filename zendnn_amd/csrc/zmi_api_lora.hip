@@ -32,6 +32,30 @@ bool lora_weights_ok(const void *p, int64_t ld, int64_t slot, int64_t n_slots, i
   return n_slots == 1 || slot >= (rows - 1) * ld + cols;
 }
 
+// Whether a row of base and a row of dst share bytes: T rows of `cols` elements of `size` bytes each.
+bool lora_rows_meet(const void *base, int64_t ld_base, const void *dst, int64_t ld_dst, int64_t T, int64_t cols, int64_t size) {
+  typedef __int128 wide;   // (strides may be anything)
+  const wide b0 = (uintptr_t)base, d0 = (uintptr_t)dst, base_step = (wide)ld_base * size, dst_step = (wide)ld_dst * size, bytes = cols * size;
+  if (b0 + (T - 1) * base_step + bytes <= d0 || d0 + (T - 1) * dst_step + bytes <= b0) return false;
+  if (base_step == dst_step || T == 1) {
+    // base's row j lies (j - i) steps and b0 - d0 from dst's row i: less than a row apart for the step below or above only
+    const wide k = T == 1 ? 0 : (d0 - b0) / base_step;
+    for (wide i = k - 1; i <= k + 1; ++i)
+      if (i > -(wide)T && i < T) {
+        const wide apart = b0 - d0 + i * base_step;
+        if (apart < bytes && -apart < bytes) return true;
+      }
+    return false;
+  }
+  for (int64_t i = 0, j = 0; i < T && j < T;) {   // (both in ascending order)
+    const wide b = b0 + j * base_step, d = d0 + i * dst_step;
+    if (b + bytes <= d) ++j;
+    else if (d + bytes <= b) ++i;
+    else return true;
+  }
+  return false;
+}
+
 ZmiLora lora_flat(const zmi_lora_t &l) {
   ZmiLora p;
   std::memset(&p, 0, sizeof(p));
@@ -81,6 +105,11 @@ int32_t zmi_lora_direct(const zmi_lora_t *l) {
   }
   if (l->ldx < l->K || l->ld_dst < cols || (l->base && l->ld_base < cols)) { set_error("lora: row stride smaller than the row"); return ZMI_FAILURE; }
   if (l->base == l->dst && l->ld_base != l->ld_dst) { set_error("lora: base at dst's address needs dst's row stride"); return ZMI_FAILURE; }
+  if (l->base && l->base != l->dst &&
+      lora_rows_meet(l->base, l->ld_base, l->dst, l->ld_dst, l->T, cols, dst_size)) {
+    set_error("lora: base and dst overlap in part (base is dst itself or apart from it)");
+    return ZMI_FAILURE;
+  }
   if ((uintptr_t)l->x % 2 || (uintptr_t)l->dst % dst_size || (uintptr_t)l->base % dst_size || (uintptr_t)l->slot_ids % 4 ||
       (uintptr_t)l->ranks % 4 || (uintptr_t)l->scales % 4 || (uintptr_t)l->workspace % 16) {
     set_error("lora: an address is not a multiple of its element's size (workspace: 16 bytes)");
