@@ -370,8 +370,12 @@ def _device_rows(name, t, dts, ndim=2):
     dt = known.get(t.dtype)
     if dt not in dts:
         raise ValueError(f"{name}: unsupported dtype {t.dtype}")
+    if max(t.shape, default=0) >= 1 << 31:   # (the argument blocks hold sizes in 32 bits)
+        raise ValueError(f"{name}: sizes of 2^31 and more are not supported")
     if not t.is_cuda:
         raise ValueError(f"{name}: not on the GPU")
+    if t.device.index != torch.cuda.current_device():   # (the library launches on the thread's current one)
+        raise ValueError(f"{name}: not on the current device")
     if t.dim() != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name}: {ndim} dimensions with a contiguous last one are required")
     return dt
@@ -421,6 +425,8 @@ def _lora_args(x, slot_ids, a, b, dst, base, ranks, scales, workspace):
     b = list(b) if isinstance(b, (list, tuple)) else [b]
     if not 1 <= len(b) <= capi.LORA_MAX_SLICES:
         raise ValueError(f"b: 1 to {capi.LORA_MAX_SLICES} slices")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace: contiguous memory is required")
     l = capi.LoraT()
     capi.load().zmi_lora_params_init(C.byref(l))
     l.dt_x = _device_rows("x", x, half)
