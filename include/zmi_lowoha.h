@@ -387,7 +387,8 @@ ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
  *   h[r]      = sum_k x[t][k] * A[a][s * rank + r][k],                            r < ranks[a]
  *   dst[t][n] = base[t][n] + scales[a] * sum_r h[r] * B_s[a][n][r]
  * Sums are f32, h goes into the second product with all bits that f32 holds (down to 2^-133), and dst is rounded once, to
- * nearest even.  An infinity or NaN in x, A or B reaches what these sums take it to, and nothing else.
+ * nearest even.  An infinity or NaN in x, A or B reaches what these sums take it to, and nothing else.  A call repeats its
+ * bits; the order of a row's sums goes by the sizes and the slot ids of the batch, not by what other rows hold.
  * base may be dst itself (same pointer and stride: the rows of dst get their adapters' part added, rows without an adapter
  * are left as they are), rows of dst's type that share no byte with dst's (failure if they do; columns of one buffer beside
  * each other are fine), or null (zero); dst overlaps no other operand.  A slot id outside [0, n_slots) means no adapter:
