@@ -397,8 +397,7 @@ ZMI_API int32_t zmi_moe_router_grouped(const zmi_moe_router_t *r);
  * x, A, B: one type, bf16 or f16; dst (and base): bf16, f16 or f32.
  * workspace: device memory of zmi_lora_workspace_size() bytes, 16-byte aligned; null: the calling thread's scratch
  * arena, which a stream that is being captured into a graph cannot use (failure) -- give a captured call a workspace that
- * no other graph shares.  T == 0 is an empty batch: success.  The size does not grow with T throughout (fewer rows may be
- * cut into more parts of K): a workspace for batches of several sizes takes the largest of their sizes.
+ * no other graph shares.  T == 0 is an empty batch: success.
  * Limits: rank <= 256, n_slices <= ZMI_LORA_MAX_SLICES, n_slots <= 4096, T <= 2^20, K <= 2^19, 2^30 columns. */
 #define ZMI_LORA_MAX_SLICES 4
 typedef struct zmi_lora_t {
@@ -418,8 +417,8 @@ typedef struct zmi_lora_t {
 } zmi_lora_t;
 /* n_slices = 1, bf16 everywhere; everything else zero. */
 ZMI_API void zmi_lora_params_init(zmi_lora_t *l);
-/* Bytes of workspace a call with these sizes (T, K, rank, n_slices, n_slots, N and the types; pointers are not looked
- * at) needs; 0 for sizes that zmi_lora_direct refuses, and for calls that need none. */
+/* Bytes of workspace that calls with these sizes (T, K, rank, n_slices, n_slots, N and the types; pointers are not looked
+ * at) and T rows or fewer need; 0 for sizes that zmi_lora_direct refuses, and for T == 0. */
 ZMI_API uint64_t zmi_lora_workspace_size(const zmi_lora_t *l);
 ZMI_API int32_t zmi_lora_direct(const zmi_lora_t *l);
 

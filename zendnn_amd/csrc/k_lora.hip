@@ -444,6 +444,9 @@ constexpr int lora_ks(int rt, int nt) { return rt + nt <= 3 ? 256 : rt + nt <= 6
 
 int64_t lora_clamp(int64_t v, int64_t lo, int64_t hi) { return v > hi ? (hi < lo ? lo : hi) : v < lo ? lo : v; }
 
+// most K slices of a small call: see lora_shape
+int64_t lora_small_slices(int64_t stages) { return lora_clamp(stages >= 16 ? stages / 4 : stages, 1, 16); }
+
 LoraShape lora_shape(const ZmiLora &p) {
   LoraShape s = {};
   s.small = p.T <= LORA_SMALL_T || (p.T <= LORA_SMALL_MOST && p.n_slots <= LORA_SMALL_SLOTS && p.rank * p.n_slices <= LORA_SMALL_RANKS);
@@ -472,7 +475,7 @@ LoraShape lora_shape(const ZmiLora &p) {
   // small: K slices of four stages or more (of one where K has few: 301 rows of K = 1001 7.6 us in four slices, 8.6 in one)
   // while there are less than two workgroups a compute unit (48 rows, 64 slots, three slices of rank 64 in eights of rank
   // tiles, both launches: 256 workgroups 23.8 us, 512 22.4, 1024 28.5)
-  s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_clamp(stages >= 16 ? stages / 4 : stages, 1, 16));
+  s.ks = (int)lora_clamp(512 / (s.tiles * s.ny), 1, lora_small_slices(stages));
   // planned: a workgroup a compute unit (two share what one already gets through: 512 workgroups 90 us against 82 for 8192
   // rows of K = 14336 at rank 128, 33 against 21 us for 2048 rows of K = 4096), runs of LORA_RUN stages or more (of two up
   // to 128 workgroups)
@@ -496,6 +499,11 @@ LoraShape lora_shape(const ZmiLora &p) {
 }
 
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+
+// workspace of a small call with that many pairs of a tile and a K slice
+size_t lora_small_bytes(const ZmiLora &p, const LoraShape &s, int64_t parts) {
+  return pad256((size_t)s.tiles * 80) + pad256((size_t)parts * p.n_slices * ((p.rank + 15) / 16) * 1024);
+}
 
 // the parts of the workspace; base null: only the size is wanted
 size_t lora_layout(const ZmiLora &p, const LoraShape &s, char *base, ZmiLoraPlan *w) {
@@ -555,6 +563,32 @@ hipError_t launch_any_shrink(const ZmiLora &p, const ZmiLoraPlan &w, const LoraS
 }
 
 }  // namespace
+
+// What no call of up to p.T rows needs more than.  Fewer rows may be cut into more parts of K, and into more or taller tiles: the
+// parts of the workspace are taken for the most that there can be.
+size_t zmi_lora_workspace_bound(const ZmiLora &p) {
+  if (p.T <= 0) return 0;
+  ZmiLora q = p;
+  size_t bytes = 0;
+  for (int32_t T : {LORA_SMALL_T, LORA_SMALL_MOST}) {
+    q.T = T < p.T ? T : p.T;
+    const LoraShape s = lora_shape(q);
+    if (!s.small) continue;
+    // (K slices times tiles: all slices of few tiles, 512 workgroups, or one slice)
+    const int64_t most = lora_small_slices((p.K + lora_ks(1, s.nt) - 1) / lora_ks(1, s.nt)), parts = lora_clamp(512 / s.ny, s.tiles, s.tiles * most);
+    const size_t n = lora_small_bytes(q, s, parts);
+    bytes = n > bytes ? n : bytes;
+  }
+  LoraShape s = lora_shape(p);
+  if (!s.small) {
+    s.rt = 4;
+    s.tiles = s.groups;
+    s.grid = 256;
+    const size_t n = lora_layout(p, s, nullptr, nullptr);
+    bytes = n > bytes ? n : bytes;
+  }
+  return bytes;
+}
 
 size_t zmi_lora_workspace_bytes(const ZmiLora &p) { return p.T > 0 ? lora_layout(p, lora_shape(p), nullptr, nullptr) : 0; }
 

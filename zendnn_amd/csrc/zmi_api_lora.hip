@@ -87,7 +87,7 @@ uint64_t zmi_lora_workspace_size(const zmi_lora_t *l) {
   clear_error();
   if (!l) { set_error("lora: null argument"); return 0; }
   if (lora_check_sizes(*l) != ZMI_SUCCESS) return 0;
-  return zmi_lora_workspace_bytes(lora_flat(*l));
+  return zmi_lora_workspace_bound(lora_flat(*l));
 }
 
 int32_t zmi_lora_direct(const zmi_lora_t *l) {

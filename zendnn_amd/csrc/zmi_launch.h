@@ -359,6 +359,7 @@ struct ZmiLoraPlan {
   int32_t n_arrivals;
 };
 size_t zmi_lora_workspace_bytes(const ZmiLora &p);   // (goes by the sizes and types only)
+size_t zmi_lora_workspace_bound(const ZmiLora &p);   // of all calls of up to T rows
 hipError_t zmi_launch_lora(const ZmiLora &p, hipStream_t stream, const char **name);
 // A1 is fragment-major over the slot numbering, K_pad = zmi_blob_kpad(H)
 hipError_t zmi_launch_moe_quant_scatter(const void *x, int64_t ldx, int T, int H, int topk,

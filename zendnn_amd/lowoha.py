@@ -467,8 +467,7 @@ def _lora_args(x, slot_ids, a, b, dst, base, ranks, scales, workspace):
 
 
 def lora_workspace_size(x, slot_ids, a, b, dst, base=None, ranks=None, scales=None):
-    """Bytes of workspace that lora_direct with these arguments needs (a shorter batch may need more: a workspace for
-    several takes the largest of their sizes)."""
+    """Bytes of workspace that lora_direct needs with these arguments, and with fewer rows."""
     return capi.load().zmi_lora_workspace_size(C.byref(_lora_args(x, slot_ids, a, b, dst, base, ranks, scales, None)))
 
 
