@@ -357,8 +357,9 @@ ZMI_API int32_t zmi_moe_router_topk(const void *logits, int32_t logits_dt, int64
  *            behind everything else; the order is that of values computed in 64 bits;
  *   weights: s of the chosen experts in that order, with renormalize != 0 divided by their sum (a zero sum leaves
  *            zeros), times scale.  A NaN logit makes the weights that it enters NaN.
- * Without a bias and groups valued by their sum the order is the logits' own, so scores that round to one value are
- * still told apart.  T == 0 is an empty batch: success.
+ * Without a bias experts (and groups, unless valued by their sum) are ordered by their logits, so scores that round to
+ * one value are still told apart.  With scoring softmax, no bias and no groups it is zmi_moe_router_topk's choice: on finite
+ * logits the same ids and weights a rounding apart, in less time.  T == 0 is an empty batch: success.
  * Limits: T <= 2^25, E <= 512, E a multiple of n_group, n_group <= 64, topk <= min(64, topk_group * E / n_group);
  * ZMI_GROUP_TOP2_SUM needs groups of two experts or more. */
 enum zmi_router_scoring { ZMI_SCORE_SOFTMAX = 0, ZMI_SCORE_SIGMOID = 1 };

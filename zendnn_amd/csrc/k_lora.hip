@@ -29,7 +29,9 @@ extern __shared__ __attribute__((aligned(16))) char lora_smem[];
 // empty places, and the shrink launch's tiles of up to `tile` rows; rows without an adapter come last.
 //
 // `waves` wavefronts of the one workgroup walk a contiguous share of the batch each, 64 rows at a time, and count per slot
-// in their own row of LDS; a row's place is its slot's count plus the number of lower lanes with the same slot.
+// in their own row of LDS; a row's place is its slot's count plus the number of lower lanes with the same slot.  Latency bounds
+// it: 5.8 us for 2048 rows of 8 slots, 11 for 8192; rows beyond those that stay in registers cost a memory latency for every 64
+// of a wavefront, 39 us for 32768 (of 2048 slots, which leave LDS for fewer wavefronts' counts: 21, 59 and 208).
 // ---------------------------------------------------------------------------------------------------------------
 #define LORA_PLAN_KEEP 8   // rows a lane keeps between the passes
 
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(1024) void zmi_lora_plan_kernel(ZmiLora p, ZmiLoraP
 // The four wavefronts share a stage as WR x WN x WK over row groups, rank tiles and 64-element blocks of K.
 //
 // What bounds it: the cache lines a compute unit can have outstanding.  In the 78 us above 4.3 M lines of 128 bytes (206 MB
-// of x, 346 MB of A read again by every tile; 77 % of the lines come from behind L2) are read with a latency of 806 clocks
+// of x, 346 MB of A read again by every tile; 71 % of the accesses that L2 counts are misses) are read with a latency of 806 clocks
 // on average, which is some 70 lines in flight in a compute unit (at 2.4 GHz); without its arithmetic the launch takes the
 // same 78 us, with all loads but the first stages' left out 54.  2048 rows of K = 4096, two slices of rank 32: 13 us for
 // 16 MB of x and A.
@@ -484,9 +486,9 @@ LoraShape lora_shape(const ZmiLora &p) {
   s.dma = p.ldx % 8 == 0 && p.a_ld % 8 == 0 && p.a_slot % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
   s.kt = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : p.rank <= 128 ? 4 : 8;
   // columns of an expand lane: eight, where the registers hold B of so many and every slice's columns are whole eights (f16,
-  // whose B takes two terms, up to rank 32, four / eight: 2593 rows of 5104 columns at rank 32 25.3 / 19.6 us, 1416 of 9480 at
-  // rank 1 20.8 / 15.9, 1937 of 2792 at rank 24 14.0 / 14.6; with rank 64 eight would gain nothing: 4096 of 4096 22.4 / 22.2,
-  // 600 of 4096 10.7 / 11.9)
+  // whose B takes two terms, up to rank 32, four / eight: 2593 rows of 5104 columns at rank 32 25.6 / 20.9 us, 1416 of 9480 at
+  // rank 1 21.5 / 17.0, 1937 of 2792 at rank 24 13.9 / 15.9; with rank 64 eight would gain nothing: 4096 of 4096 24.8 / 25.4,
+  // 600 of 4096 11.2 / 13.0)
   bool eights = !s.small && p.dt_dst != ZMI_DT_F32 && s.kt <= (p.dt_x == ZMI_DT_BF16 ? 4 : 1);
   for (int i = 0; i < p.n_slices; ++i) eights &= p.N[i] % 8 == 0;
   s.nj = s.kt == 8 ? 2 : eights ? 8 : 4;

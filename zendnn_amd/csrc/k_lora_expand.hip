@@ -5,8 +5,9 @@
 // of a row.  (With the operands the other way round 16 neighbouring lanes stand in 16 rows, and the address path of the
 // compute unit takes four times as long over every access.)
 //
-// HBM bounds it: base and dst once, B and h from L2 (2048 rows, 2 x 14336 columns, rank 32: 235 MB of base and dst in 50 us,
-// 4.7 TB/s where a large copy reaches 4.9; 8192 rows, 4096 columns, rank 128: 39 us).  Planned calls run down the 16-row groups of the batch with B in
+// HBM bounds it: base and dst once, B and h from L2 (2048 rows, 2 x 14336 columns, rank 32: 235 MB of base and dst in 51 us,
+// 4.6 TB/s where a large copy reaches 4.9; 8192 rows, 4096 columns, rank 128: 43 us, of which three terms of h instead of two
+// are 2 to 3).  Planned calls run down the 16-row groups of the batch with B in
 // registers, reloaded where the slot changes; each workgroup takes an equal share of the groups, h of the next group goes
 // to LDS and its base to registers while one is computed, and a group's stores go out behind the next group's loads.
 #include <type_traits>
@@ -295,8 +296,8 @@ __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_kernel(Zmi
 }
 
 // Calls without a plan launch: workgroup (x: columns of a slice, y: tile of up to 16 rows); h comes as the K slices' sums.
-// Latency bounds it, the chain from the tile's entry over B and the sums to dst: 4.6 us for one row of 4096 columns at rank
-// 16, 10 us for 48 rows of 6144 columns at rank 64, whose B alone is 16 MB.
+// Latency bounds it, the chain from the tile's entry over B and the sums to dst: 4.9 us for one row of 4096 columns at rank
+// 16, 10.4 us for 48 rows of 6144 columns at rank 64, whose B alone is 16 MB.
 template <bool F16, int NJ, int KT, int DST>
 __global__ __launch_bounds__(LORA_WAVES * 64, 2) void zmi_lora_expand_small_kernel(ZmiLora p, ZmiLoraPlan w, int slices) {
   typedef Out<NJ, DST> O;

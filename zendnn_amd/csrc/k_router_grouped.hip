@@ -10,14 +10,15 @@
 // Two experts of one token can lie nearer to each other than f32 tells apart (256 experts leave gaps of 1e-3 on average,
 // so one token in some hundreds has two chosen or bordering values within f32's error), and ids have to be those of
 // exact values.  The choice is therefore made on f32 values while every gap that decides it -- between one chosen expert
-// and the next, the last and the best that is left, the last group and the best that is left -- is wider than twice what
+// and the next, the last and the best that is left, the last group and the best that is left -- is wider than what
 // the f32 values can be off by; a token where one is not is chosen again by the same rounds on 64-bit values.  Without a
 // bias experts are ordered by their logits, exactly, and no score is computed but those of the chosen.
 //
-// What bounds it: instructions.  8192 tokens of 256 f32 logits (sigmoid, bias, 4 of 8 groups, 8 experts) take 12.0 us and
-// 605 vector instructions a token, 32768 of 512 (softmax, bias, 10 experts) 37.9 us and 719, where the bytes alone would
-// take 2 and 14 us; at four clocks an instruction and 2.4 GHz that is 8 and 38 us.  Short batches are a launch and one
-// token's chain: 4 us.
+// What bounds it: instructions.  8192 tokens of 256 f32 logits (sigmoid, bias, 4 of 8 groups, 8 experts) take 12.8 us and
+// 621 vector instructions a token, 32768 of 512 (softmax, bias, 10 experts) 38 us and 761, where the bytes alone would
+// take 2 and 14 us; at four clocks an instruction and 2.4 GHz that would be 8 and 41 us.  Short batches are a launch and one
+// token's chain: 4 us.  Logits with many equal values under an equal bias have most tokens chosen twice: 8192 x 256 bf16
+// with a zero bias 19.6 us, with a random one 13.0.
 #include <type_traits>
 
 #include "zmi_device.h"
