@@ -123,3 +123,26 @@ def test_h_keeps_24_bits(T, dt, dst):
     want = (h + c.base.double()).to(dst)
     assert c.call(c.base) == capi.SUCCESS, lowoha.last_error()
     assert torch.equal(c.dst, want), float((c.dst.double() - want.double()).abs().max())
+
+
+@pytest.mark.parametrize("T", [40, 700])
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("others", [0.0, 1.0])
+def test_rows_that_are_not_finite_from_some_rank_on(T, dt, others):
+    """One infinite (or NaN) element of x per row, which A's row r reads with weight 2 and the others with `others`: at 0 their h
+    is NaN in front of, between and behind what rank r holds, at 1 all of h is infinite."""
+    c = Case(T, T, 192, [40], 37, 3, dt, F32, mixed=False, none=0.0)
+    c.scales = c.scales.abs() + 0.25
+    c.b[0].abs_().add_(2.0 ** -6)
+    c.x[:, 5] = 0.0
+    clean, rows = c.x.clone(), [1, 17, T - 1]
+    for value in (float("nan"), INF, -INF):
+        for r in (0, 7, 8, 31, 32, 36):
+            c.x.copy_(clean)
+            c.x[rows, 5] = value
+            c.a[:, :, 5] = others
+            c.a[:, r, 5] = 2.0
+            y = definition(c, None)
+            assert not torch.isfinite(y[rows]).any()
+            assert c.call(None) == capi.SUCCESS, lowoha.last_error()
+            same_kind(c.dst, y)
